@@ -149,9 +149,10 @@ def _inputs(case, seed):
 
 
 class _DeviceArray:
-    """a kept tensor of the framework's device, left where it is"""
+    """a kept tensor of the framework's device, left where it is; the memory belongs to the device's handle"""
 
-    def __init__(self, address, shape):
+    def __init__(self, device, address, shape):
+        self.device = device
         self.__cuda_array_interface__ = dict(shape=tuple(shape), typestr="<f4", data=(address, False), version=2)
 
 
@@ -220,7 +221,7 @@ def run(state):
     if own:
         p = state["program"]
         p["device"].execute_blob(p["blob"])
-        return [torch.as_tensor(_DeviceArray(*p["device"].get_tensor_device(i)), device="cuda") for i in p["ids"]]
+        return [torch.as_tensor(_DeviceArray(p["device"], *p["device"].get_tensor_device(i)), device="cuda") for i in p["ids"]]
     case, x = state["case"], state["x"]
     if case["op"] == "norm":
         return _norm(case, x)
