@@ -81,6 +81,9 @@ class _State:
     device = None
     dep: set | None = None
     harsh = False
+    waiting: dict = {}     # operators that have received gradients in the backward pass under way, by creation order
+    passes = 0             # depth of Tensor.backward calls under way
+    operators = 0          # operators created so far
 
 
 def _irb() -> _IRBase:
@@ -225,7 +228,16 @@ class Tensor:
         return self.n.forward()
 
     def backward(self):
-        self.n.backward(Value.ones(self.dim()))
+        _State.passes += 1
+        try:
+            self.n.backward(Value.ones(self.dim()))
+            while _State.waiting:
+                # the operator created last cannot feed one created before it: its gradients are complete
+                _State.waiting.pop(max(_State.waiting)).emit_gradients()
+        finally:
+            _State.passes -= 1
+            if not _State.passes:
+                _State.waiting.clear()
 
     def dim(self) -> list:
         return self.n.dim()
@@ -825,6 +837,199 @@ def bmm(a: Tensor, b: Tensor) -> Tensor:
 
 
 # --------------------------------------------------------------------------------------
+# operators of transformer layers (IR extensions; upstream composes its layers from the nodes above,
+# src/nn/transformer.rs:10-40, src/nn/norm/rms.rs)
+# --------------------------------------------------------------------------------------
+class _Operator:
+    """One operator command with its results.  Gradients that arrive at the results are summed up and leave in one
+    gradient command: inside `Tensor.backward` once every operator created later has sent its own, so that an operator
+    whose results are used several times runs its backward once; elsewhere at once."""
+
+    CMD = None
+
+    def __init__(self, args, ints, reals):
+        self.args, self.ints, self.reals = list(args), list(ints), list(reals)
+        self.order = _State.operators
+        _State.operators += 1
+        self.vals = None
+        self.grads = None
+
+    def dims(self) -> list:
+        """shapes of the results"""
+        raise NotImplementedError
+
+    def emit_backward(self, grads):
+        raise NotImplementedError
+
+    def ready(self):
+        return self.vals is not None and all(a is None or a.val() is not None for a in self.args)
+
+    def forward(self):
+        if not self.ready():
+            ids = [None if a is None else a.forward().id for a in self.args]
+            outs = [v.id for v in self.vals] if self.vals is not None else [ir_b_id() for _ in self.dims()]
+            ir_b_add((self.CMD, ids, outs, self.ints, self.reals))
+            self.vals = [Value(d, o) for d, o in zip(self.dims(), outs)]
+        return self.vals
+
+    def take_gradient(self, k, grad: Value):
+        assert self.vals is not None, "forward first"
+        if self.grads is None:
+            self.grads = [None] * len(self.vals)
+        old = self.grads[k]
+        # a value of its own: by the time it is used, a leaf may have summed other gradients up in the same id
+        self.grads[k] = (grad.to_node().contigious() if old is None else old.to_node() + grad.to_node()).forward()
+        if _State.passes:
+            _State.waiting[self.order] = self
+        else:
+            self.emit_gradients()
+
+    def emit_gradients(self):
+        grads, self.grads = self.grads, None
+        self.emit_backward(grads)
+
+    def arg_ids(self):
+        return [None if a is None else a.val().id for a in self.args]
+
+
+class OperatorNode(Node):
+    """result `k` of an operator"""
+
+    def __init__(self, op: _Operator, k: int = 0):
+        self.op, self.k = op, k
+
+    def forward(self): return self.op.forward()[self.k].clone()
+    def backward(self, grad): self.op.take_gradient(self.k, grad)
+    def dim(self): return list(self.op.dims()[self.k])
+    def val(self): return self.op.vals[self.k].clone() if self.op.ready() else None
+
+
+class _RmsNorm(_Operator):
+    CMD = "RmsNorm"
+
+    def dims(self): return [self.args[0].dim()] * 2
+
+    def emit_backward(self, grads):
+        x, scale, residual = self.args
+        dy, dh = grads
+        if dy is None:
+            dx = dh
+        else:
+            h = self.vals[1]
+            dx, dscale = Value(h.dim, ir_b_id()), Value(scale.dim(), ir_b_id())
+            ir_b_add(("RmsNormGrad", [h.id, scale.val().id, dy.id, None if dh is None else dh.id], [dx.id, dscale.id],
+                      [], self.reals))
+            scale.n.backward(dscale)
+        if residual is not None:
+            # a value of its own: gradients that reach x later must not show up in the residual's
+            residual.n.backward(dx.to_node().contigious().forward())
+        x.n.backward(dx)
+
+
+def rms_norm(x: Tensor, scale: Tensor, residual: Tensor = None, eps: float = 1e-6):
+    """`y = h / sqrt(mean(h^2) + eps) * scale` over the last axis with `h = x + residual`, in one pass.  Returns y, or
+    (y, h) when a residual is given (h is the next layer's residual)."""
+    width = x.dim()[-1:]
+    if width in ([], [0]):
+        raise ValueError("rms_norm needs an axis with elements")
+    if scale.dim() != width:
+        raise ValueError(f"rms_norm: the scale must be {width}, not {scale.dim()}")
+    if residual is not None and residual.dim() != x.dim():
+        raise ValueError(f"rms_norm: the residual must be {x.dim()}, not {residual.dim()}")
+    if not eps >= 0:
+        raise ValueError("rms_norm: eps must not be negative")
+    op = _RmsNorm([x, scale, residual], [], [float(eps)])
+    y = Tensor(OperatorNode(op, 0))
+    return y if residual is None else (y, Tensor(OperatorNode(op, 1)))
+
+
+class _Rotary(_Operator):
+    CMD = "Rotary"
+
+    def dims(self): return [self.args[0].dim()]
+
+    def emit_backward(self, grads):
+        x, table, positions = self.args
+        dx = Value(x.dim(), ir_b_id())
+        ints = [self.ints[0], 1 - self.ints[1], self.ints[2]]
+        ir_b_add((self.CMD, [grads[0].id] + self.arg_ids()[1:], [dx.id], ints, self.reals))
+        x.n.backward(dx)
+
+
+def rotary(x: Tensor, table: Tensor, positions: Tensor = None, offset: int = 0, interleaved: bool = False,
+           gain: float = 1.0) -> Tensor:
+    """Turns the first 2 P elements of every head of `x` [batch, tokens, heads, head size] by angles that grow with the
+    token's position: `positions` ([tokens] or [batch, tokens], whole numbers) or offset + token.  `table` [2, P] holds
+    each pair's frequency in whole turns per position as the sum of two floats (`nn.Rotary` makes it).  A pair is two
+    neighbours (`interleaved`) or elements i and P + i.  No gradient flows into the table and the positions."""
+    d, t = x.dim(), table.dim()
+    if len(d) != 4:
+        raise ValueError("rotary needs [batch, tokens, heads, head size]")
+    if len(t) != 2 or t[0] != 2 or not 1 <= t[1] <= min(d[3] // 2, 4096):
+        raise ValueError(f"rotary: a table {t} does not fit heads of {d[3]} elements")
+    if positions is not None and positions.dim() not in ([d[1]], d[:2]):
+        raise ValueError(f"rotary: positions must be [tokens] or [batch, tokens], not {positions.dim()}")
+    if positions is not None and offset:
+        raise ValueError("rotary: positions and an offset exclude one another")
+    if abs(offset) > 1 << 24 or int(offset) != offset:
+        raise ValueError("rotary: the offset must be a whole number within 2^24")
+    return Tensor(OperatorNode(_Rotary([x, table, positions], [int(bool(interleaved)), 0, int(offset)], [float(gain)])))
+
+
+class _Attention(_Operator):
+    CMD = "Attention"
+
+    def dims(self):
+        q = self.args[0].dim()
+        return [q, [q[0], q[2], q[1]]]
+
+    def emit_backward(self, grads):
+        out, lse = self.vals
+        d = [Value(self.args[i].dim(), ir_b_id()) for i in range(3)]
+        ir_b_add(("AttentionGrad", self.arg_ids() + [out.id, lse.id, grads[0].id], [v.id for v in d], self.ints, self.reals))
+        for a, v in zip(self.args, d):
+            a.n.backward(v)
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, scale: float = None, causal: bool = True, cap: float = 0.0,
+              slopes: Tensor = None, docs: Tensor = None, prefix: Tensor = None, lengths: Tensor = None) -> Tensor:
+    """softmax(scores) . v without ever holding the scores: q [batch, queries, heads, size], k and v [batch, keys, key
+    heads, size], the query heads a multiple of the key heads (neighbouring query heads share one).  The queries are the
+    last positions of their sequence.
+
+    scale    of the products (1 / sqrt(size)); cap: scores become cap * tanh(score / cap)
+    causal   a query sees the keys up to its own position
+    slopes   [heads]: slope * distance between query and key is subtracted from a score
+    docs     [batch, keys]: a query sees only keys with the document number of its own position; negative: padding
+    prefix   [batch]: the first keys of a sequence, which every query sees in spite of the causal mask
+    lengths  [batch]: how many keys of the cache a sequence has; the rest is not read
+
+    A query that sees nothing gives zeros.  No gradient flows into slopes, docs, prefix and lengths."""
+    dq, dk = q.dim(), k.dim()
+    if len(dq) != 4 or len(dk) != 4 or v.dim() != dk:
+        raise ValueError(f"attention: operands {dq}, {dk}, {v.dim()} are not [batch, tokens, heads, size]")
+    if dq[0] != dk[0] or dq[3] != dk[3]:
+        raise ValueError("attention: queries and keys differ in their batch or head size")
+    if not 1 <= dq[3] <= 256:
+        raise ValueError("attention: the head size must lie between 1 and 256")
+    if dq[2] < 1 or dk[2] < 1 or dq[2] % dk[2]:
+        raise ValueError("attention: the query heads must be a multiple of the key heads")
+    if max(dq[1], dk[1]) >= 1 << 24:
+        raise ValueError("attention: more than 2^24 tokens")
+    for what, t, want in (("slopes", slopes, [dq[2]]), ("docs", docs, dk[:2]), ("prefix", prefix, dq[:1]), ("lengths", lengths, dq[:1])):
+        if t is not None and t.dim() != want:
+            raise ValueError(f"attention: {what} must be {want}, not {t.dim()}")
+    if docs is not None and dq[1] > dk[1]:
+        raise ValueError("attention: with docs there cannot be more queries than keys")
+    if prefix is not None and not causal:
+        raise ValueError("attention: a prefix only means something under the causal mask")
+    scale = 1.0 / math.sqrt(dq[3]) if scale is None else float(scale)
+    if not math.isfinite(scale) or not (math.isfinite(cap) and cap >= 0):
+        raise ValueError("attention: scale and cap must be finite, the cap not negative")
+    return Tensor(OperatorNode(_Attention([q, k, v, slopes, docs, prefix, lengths], [int(bool(causal))], [scale, float(cap)])))
+
+
+# --------------------------------------------------------------------------------------
 # data-movement nodes (src/graph/data)
 # --------------------------------------------------------------------------------------
 def handle_minus_dim(source_dim, input_dim):
@@ -1121,6 +1326,7 @@ def set_device(device):
     _State.device = device
     _State.dep = set()
     _State.harsh = False
+    _State.waiting = {}
 
 
 def add_heading(cmt: str):

@@ -20,7 +20,30 @@ enum Op : uint8_t {
     OP_WHILE = 23, OP_IF = 24, OP_EX = 25, OP_HEADING = 26, OP_ALLREDUCE = 27,
     OP_MAX = 28,  // extension: row maximum of a 2-d tensor, same shape contract as OP_SUM
     OP_BATCH_DOT = 29,  // extension: [B,M,K] x [B,K,N] -> [B,M,N]
+    // extensions: the operators of transformer layers.  Each takes a list of operands (some optional), gives a list of
+    // results and carries whole and real parameters; operator_signature() says how many of each.
+    OP_RMS_NORM = 30, OP_RMS_NORM_GRAD = 31, OP_ROTARY = 32, OP_ATTENTION = 33, OP_ATTENTION_GRAD = 34,
 };
+
+constexpr uint32_t NO_ID = 0xffffffffu;   // an optional operand that is absent
+
+struct OperatorSignature {
+    uint32_t args, required;   // operands, and how many of the first must be present
+    uint32_t outs, ints, reals;
+    uint32_t also_required;    // bit i: operand i must be present although an optional one stands before it
+};
+// operands and results in the order of include/adb200.h; args == 0: not an operator
+inline OperatorSignature operator_signature(uint8_t op) {
+    switch (op) {
+    case OP_RMS_NORM: return {3, 2, 2, 0, 1, 0};
+    case OP_RMS_NORM_GRAD: return {4, 3, 2, 0, 1, 0};
+    case OP_ROTARY: return {3, 2, 1, 3, 1, 0};
+    case OP_ATTENTION: return {7, 3, 2, 1, 2, 0};
+    case OP_ATTENTION_GRAD: return {10, 3, 3, 1, 2, (1u << 7) | (1u << 8) | (1u << 9)};
+    default: return {0, 0, 0, 0, 0, 0};
+    }
+}
+inline bool is_operator(uint8_t op) { return operator_signature(op).args > 0; }
 
 enum PayloadKind : uint8_t { PAYLOAD_INLINE = 0, PAYLOAD_HOST = 1, PAYLOAD_DEVICE = 2 };
 
@@ -41,7 +64,16 @@ struct Cmd {
     std::vector<std::pair<uint32_t, std::unique_ptr<Block>>> conds;  // If
     std::unique_ptr<Block> else_block;
     std::string text;               // Heading
+    std::vector<uint32_t> args, outs;  // operators: operands (NO_ID where absent) and results; res = outs[0]
+    std::vector<int64_t> ints;
+    std::vector<float> reals;
 };
+
+// the results of a command, one after another
+template <class F> inline void each_result(const Cmd& c, F&& f) {
+    if (c.outs.empty()) f(c.res);
+    else for (uint32_t o : c.outs) f(o);
+}
 
 struct Block {
     std::vector<Cmd> cmds;
@@ -159,6 +191,28 @@ inline void parse_cmd(Reader& r, Program& prog, Cmd& c, int depth) {
     case OP_EX: break;
     case OP_HEADING: c.text = r.str(r.get<uint16_t>()); break;
     case OP_ALLREDUCE: c.a = id(); c.res = c.a; break;
+    case OP_RMS_NORM: case OP_RMS_NORM_GRAD: case OP_ROTARY: case OP_ATTENTION: case OP_ATTENTION_GRAD: {
+        const OperatorSignature sig = operator_signature(c.op);
+        if (r.get<uint8_t>() != sig.args) throw IrError("operator with a wrong number of operands");
+        for (uint32_t i = 0; i < sig.args; i++) {
+            uint32_t v = r.get<uint32_t>();
+            if (v == NO_ID ? (i < sig.required || (sig.also_required >> i & 1)) : v >= prog.ids.size())
+                throw IrError("id index out of range");
+            c.args.push_back(v);
+        }
+        if (r.get<uint8_t>() != sig.outs) throw IrError("operator with a wrong number of results");
+        for (uint32_t i = 0; i < sig.outs; i++) {
+            c.outs.push_back(id());
+            for (uint32_t k = 0; k < i; k++)
+                if (c.outs[k] == c.outs[i]) throw IrError("operator with the same id for two results");
+        }
+        c.res = c.outs[0];
+        if (r.get<uint8_t>() != sig.ints) throw IrError("operator with a wrong number of parameters");
+        for (uint32_t i = 0; i < sig.ints; i++) c.ints.push_back(r.get<int64_t>());
+        if (r.get<uint8_t>() != sig.reals) throw IrError("operator with a wrong number of parameters");
+        for (uint32_t i = 0; i < sig.reals; i++) c.reals.push_back(r.get<float>());
+        break;
+    }
     default: throw IrError("unknown opcode " + std::to_string(int(c.op)));
     }
     prog.n_cmds++;
@@ -246,6 +300,16 @@ inline void write_cmd(Writer& w, const Cmd& c, std::vector<std::pair<size_t, con
         w.buf.insert(w.buf.end(), c.text.begin(), c.text.end());
         break;
     case OP_ALLREDUCE: w.put<uint32_t>(c.a); break;
+    default:   // operators
+        w.put<uint8_t>(uint8_t(c.args.size()));
+        for (auto a : c.args) w.put<uint32_t>(a);
+        w.put<uint8_t>(uint8_t(c.outs.size()));
+        for (auto o : c.outs) w.put<uint32_t>(o);
+        w.put<uint8_t>(uint8_t(c.ints.size()));
+        for (auto i : c.ints) w.put<int64_t>(i);
+        w.put<uint8_t>(uint8_t(c.reals.size()));
+        for (auto f : c.reals) w.put<float>(f);
+        break;
     }
 }
 

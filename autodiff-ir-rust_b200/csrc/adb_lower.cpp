@@ -8,6 +8,7 @@
 #include "adb_lower.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <limits>
 #include <map>
@@ -55,9 +56,13 @@ bool has_result(uint8_t op) {
     }
 }
 
+constexpr int MAX_READS = 10;   // the operator with the most operands
+
 // operands read by a command (in-place forms also read their target)
-void cmd_reads(const Cmd& c, uint32_t out[2], int& n) {
+void cmd_reads(const Cmd& c, uint32_t out[MAX_READS], int& n) {
     n = 0;
+    for (uint32_t a : c.args)
+        if (a != NO_ID) out[n++] = a;
     switch (c.op) {
     case OP_MUL: case OP_ADD: case OP_DOT: case OP_BATCH_DOT: case OP_CONCAT: case OP_MUL_EQ: case OP_ADD_EQ:
         out[n++] = c.a; out[n++] = c.b; break;
@@ -175,7 +180,7 @@ class Lowerer {
             else if (c.op == OP_IF) {
                 for (auto& cb : c.conds) nested(*cb.second);
                 if (c.else_block) nested(*c.else_block);
-            } else if (has_result(c.op)) out.push_back(c.res);
+            } else if (has_result(c.op)) each_result(c, [&](uint32_t id) { out.push_back(id); });
         }
         std::sort(out.begin(), out.end());
         out.erase(std::unique(out.begin(), out.end()), out.end());
@@ -215,7 +220,7 @@ class Lowerer {
             return out;
         }
         if (!has_result(c.op) || !live(c)) return st;
-        uint32_t r[2];
+        uint32_t r[MAX_READS];
         int n;
         cmd_reads(c, r, n);
         for (int k = 0; k < n; k++) {
@@ -223,8 +228,13 @@ class Lowerer {
             if (is_alias_op(c.op)) { if (c.res != f.id) f.readers.insert(c.res); }
             else scan_read(r[k], st, f);
         }
-        if (c.res == f.id) return S_REBOUND;
-        if (f.sources.count(c.res) && (st & S_WINDOW)) st = uint8_t((st & ~S_WINDOW) | S_STALE);
+        bool rebound = false, stale = false;
+        each_result(c, [&](uint32_t id) {
+            if (id == f.id) rebound = true;
+            else if (f.sources.count(id)) stale = true;
+        });
+        if (rebound) return S_REBOUND;
+        if (stale && (st & S_WINDOW)) st = uint8_t((st & ~S_WINDOW) | S_STALE);
         return st;
     }
     uint8_t scan_cmds(const Block& b, size_t from, uint8_t st, FreezeScan& f) {
@@ -323,11 +333,11 @@ class Lowerer {
                 if (c.else_block) analyze(*c.else_block, seg);
                 cur = ++seg;
             } else if (has_result(c.op)) {
-                uint32_t r[2];
+                uint32_t r[MAX_READS];
                 int n;
                 cmd_reads(c, r, n);
                 for (int k = 0; k < n; k++) use(r[k], cur);
-                def(c.res, cur);
+                each_result(c, [&](uint32_t id) { def(id, cur); });
                 if (c.op == OP_ALLREDUCE) info_[c.a].cross = true;
             }
         }
@@ -346,8 +356,8 @@ class Lowerer {
                 else if (c.op == OP_IF) {
                     for (auto& cb : c.conds) walk(*cb.second);
                     if (c.else_block) walk(*c.else_block);
-                } else if (has_result(c.op) && info_[c.res].needed) {
-                    uint32_t r[2];
+                } else if (has_result(c.op) && live(c)) {
+                    uint32_t r[MAX_READS];
                     int n;
                     cmd_reads(c, r, n);
                     for (int k = 0; k < n; k++)
@@ -360,7 +370,12 @@ class Lowerer {
             walk(prog_.main);
         }
     }
-    bool live(const Cmd& c) const { return !has_result(c.op) || info_[c.res].needed; }
+    bool live(const Cmd& c) const {
+        if (!has_result(c.op)) return true;
+        bool any = false;
+        each_result(c, [&](uint32_t id) { any = any || info_[id].needed; });
+        return any;
+    }
 
     void count_uses(Block& b) {
         for (auto& c : b.cmds) {
@@ -369,7 +384,7 @@ class Lowerer {
                 for (auto& cb : c.conds) { info_[cb.first].uses += 1; count_uses(*cb.second); }
                 if (c.else_block) count_uses(*c.else_block);
             } else if (has_result(c.op) && live(c)) {
-                uint32_t r[2];
+                uint32_t r[MAX_READS];
                 int n;
                 cmd_reads(c, r, n);
                 for (int k = 0; k < n; k++) info_[r[k]].uses++;
@@ -971,6 +986,10 @@ class Lowerer {
         case OP_DOT: return lower_dot(c);
         case OP_BATCH_DOT: return lower_batch_dot(c);
         case OP_ALLREDUCE: return lower_allreduce(c);
+        case OP_RMS_NORM: return lower_rms_norm(c);
+        case OP_RMS_NORM_GRAD: return lower_rms_norm_grad(c);
+        case OP_ROTARY: return lower_rotary(c);
+        case OP_ATTENTION: case OP_ATTENTION_GRAD: return lower_attention(c);
         default: fail("internal: unexpected command in straight-line code");
         }
     }
@@ -1375,6 +1394,215 @@ class Lowerer {
         else bind_own_buffer(c.res, buf, rs);
     }
 
+    // ------------------------------------------------------------------ operators of transformer layers
+    using Access = Step::Oper::Access;
+
+    // an operand read where it lies: any strides, as long as every axis is one run and the last one is contiguous
+    // (a broadcast axis has stride 0); anything else is written out first
+    Access operand_access(Node* n) {
+        n = g_.canon(n);
+        const size_t nd = n->shape.size();
+        bool ok = n->kind == N_LOAD;
+        for (size_t d = 0; ok && d < nd; d++) ok = n->view.dims[d].size() <= 1;
+        Access a;
+        if (ok) {
+            for (size_t d = 0; d < nd; d++) a.stride.push_back(n->view.dims[d].empty() ? 0 : n->view.dims[d][0].stride);
+            ok = n->shape[nd - 1] == 1 || a.stride[nd - 1] == 1;
+        }
+        if (ok) {
+            a.buf = n->buf;
+            a.off = n->view.offset;
+            return a;
+        }
+        Node* m = materialize_node(n);
+        a.buf = m->buf;
+        a.off = m->view.offset;   // a value that lies in memory contiguously is not copied
+        a.stride.assign(nd, 1);
+        for (size_t d = nd - 1; d-- > 0;) a.stride[d] = a.stride[d + 1] * n->shape[d + 1];
+        return a;
+    }
+    // the operand as one contiguous run
+    Access flat_operand(Node* n) {
+        Node* m = materialize_node(n);
+        Access a;
+        a.buf = m->buf;
+        a.off = m->view.offset;
+        return a;
+    }
+    // [..., width] as rows of `width`
+    Access row_operand(Node* n, int64_t rows, int64_t width) {
+        Node* r = g_.reshape(n, {rows, width});
+        if (!r) r = g_.reshape(materialize_node(n), {rows, width});
+        if (!r) fail("internal: rows of a contiguous value");
+        return operand_access(r);
+    }
+    Node* operand(const Cmd& c, size_t i) { return c.args[i] == NO_ID ? nullptr : resolve(c.args[i]); }
+    void consume_args(const Cmd& c) {
+        for (uint32_t a : c.args)
+            if (a != NO_ID) consume(a);
+    }
+
+    // Pushes the step.  Every result that something needs gets a buffer that no operand lies in.  The operands are
+    // looked up (`operands`) only after the buffers have been cleared of values that others still read, while the
+    // command still counts as a reader of them: writing those values out may move them.
+    template <class F>
+    void push_oper(const Cmd& c, F&& operands, const std::vector<Shape>& out_shapes, std::vector<int64_t> dims, int64_t work) {
+        std::vector<int> bufs(c.outs.size(), -1);
+        std::vector<char> apart(c.outs.size(), 0);
+        for (size_t k = 0; k < c.outs.size(); k++)
+            if (info_[c.outs[k]].needed) bufs[k] = result_buffer(c.outs[k], out_shapes[k]);
+        for (int b : bufs)
+            if (b >= 0) before_write(b, c.outs);
+        std::vector<Access> in = operands();
+        consume_args(c);
+        for (size_t k = 0; k < c.outs.size(); k++) {
+            for (auto& a : in) apart[k] = apart[k] || (bufs[k] >= 0 && a.buf == bufs[k]);
+            if (apart[k]) bufs[k] = temp_buffer(numel(out_shapes[k]));
+        }
+        const int wbuf = work > 0 ? temp_buffer(work) : -1;
+        Step& s = push_step(Step::OPER);
+        s.oper.op = c.op;
+        s.oper.in = std::move(in);
+        s.oper.dims = std::move(dims);
+        s.oper.ints = c.ints;
+        s.oper.reals = c.reals;
+        s.oper.work = wbuf;
+        for (auto& a : s.oper.in)
+            if (a.buf >= 0) touch(a.buf, s.pos);
+        if (wbuf >= 0) touch(wbuf, s.pos);
+        for (size_t k = 0; k < c.outs.size(); k++) {
+            Access a;
+            a.buf = bufs[k];
+            s.oper.out.push_back(a);
+            if (bufs[k] < 0) continue;
+            touch(bufs[k], s.pos);
+            g_.buf_version[size_t(bufs[k])]++;
+            if (apart[k]) bind_value(c.outs[k], g_.load(bufs[k], out_shapes[k], contiguous_view(out_shapes[k])));
+            else bind_own_buffer(c.outs[k], bufs[k], out_shapes[k]);
+        }
+    }
+    void bind_result(const Cmd& c, size_t k, float v, const Shape& shape) {
+        if (info_[c.outs[k]].needed) after_op(c.outs[k], g_.constant(v, shape));
+    }
+
+    void lower_rms_norm(const Cmd& c) {
+        Node *x = operand(c, 0), *scale = operand(c, 1), *res = operand(c, 2);
+        if (x->shape.empty() || x->shape.back() == 0) fail("RmsNorm of '" + name(c.args[0]) + "': the last axis has no elements");
+        const int64_t width = x->shape.back(), rows = numel(x->shape) / width;
+        if (scale->shape != Shape{width}) fail("RmsNorm: the scale must have one value for each element of the last axis");
+        if (res && res->shape != x->shape) fail("RmsNorm: the residual must have the operand's shape");
+        if (!(c.reals[0] >= 0.f)) fail("RmsNorm: eps must not be negative");
+        const Shape shape = x->shape;
+        if (rows == 0) {
+            consume_args(c);
+            for (size_t k = 0; k < 2; k++) bind_result(c, k, 0.f, shape);
+            return;
+        }
+        push_oper(c, [&] {
+            return std::vector<Access>{row_operand(operand(c, 0), rows, width), flat_operand(operand(c, 1)),
+                                       res ? row_operand(operand(c, 2), rows, width) : Access{}};
+        }, {shape, shape}, {rows, width}, 0);
+    }
+
+    void lower_rms_norm_grad(const Cmd& c) {
+        Node *h = operand(c, 0), *scale = operand(c, 1), *dy = operand(c, 2), *dh = operand(c, 3);
+        if (h->shape.empty() || h->shape.back() == 0) fail("RmsNormGrad of '" + name(c.args[0]) + "': the last axis has no elements");
+        const int64_t width = h->shape.back(), rows = numel(h->shape) / width;
+        if (scale->shape != Shape{width}) fail("RmsNormGrad: the scale must have one value for each element of the last axis");
+        if (dy->shape != h->shape || (dh && dh->shape != h->shape)) fail("RmsNormGrad: gradients must have the operand's shape");
+        if (!(c.reals[0] >= 0.f)) fail("RmsNormGrad: eps must not be negative");
+        const Shape shape = h->shape;
+        if (rows == 0) {
+            consume_args(c);
+            bind_result(c, 0, 0.f, shape);
+            bind_result(c, 1, 0.f, {width});
+            return;
+        }
+        push_oper(c, [&] {
+            return std::vector<Access>{row_operand(operand(c, 0), rows, width), flat_operand(operand(c, 1)),
+                                       row_operand(operand(c, 2), rows, width), dh ? row_operand(operand(c, 3), rows, width) : Access{}};
+        }, {shape, {width}}, {rows, width}, norm_grad_workspace(rows, width, opt_.sm_count));
+    }
+
+    void lower_rotary(const Cmd& c) {
+        Node *x = operand(c, 0), *table = operand(c, 1), *pos = operand(c, 2);
+        if (x->shape.size() != 4) fail("Rotary needs an operand [batch, tokens, heads, head size]");
+        if (table->shape.size() != 2 || table->shape[0] != 2) fail("Rotary needs a table [2, pairs]");
+        const Shape s = x->shape;
+        const int64_t pairs = table->shape[1];
+        if (pairs < 1 || 2 * pairs > s[3]) fail("Rotary turns between one pair and the whole head");
+        if (pairs > ROTARY_MAX_PAIRS || s[2] * s[3] > (int64_t(1) << 28)) fail("Rotary: more than " + std::to_string(ROTARY_MAX_PAIRS) + " pairs or 2^28 elements a token");
+        if (pos && pos->shape != Shape{s[1]} && pos->shape != Shape{s[0], s[1]}) fail("Rotary: positions must be [tokens] or [batch, tokens]");
+        for (int k = 0; k < 2; k++)
+            if (c.ints[size_t(k)] != 0 && c.ints[size_t(k)] != 1) fail("Rotary: a flag that is neither 0 nor 1");
+        if (c.ints[2] < -(int64_t(1) << 24) || c.ints[2] > (int64_t(1) << 24)) fail("Rotary: the first position is beyond 2^24");
+        if (numel(s) == 0) {
+            consume_args(c);
+            bind_result(c, 0, 0.f, s);
+            return;
+        }
+        push_oper(c, [&] {
+            Access at;
+            if (pos) {
+                at = operand_access(operand(c, 2));
+                if (at.stride.size() == 1) at.stride.insert(at.stride.begin(), 0);
+            }
+            return std::vector<Access>{operand_access(operand(c, 0)), flat_operand(operand(c, 1)), at};
+        }, {s}, {s[0], s[1], s[2], s[3], pairs}, 0);
+    }
+
+    // Attention and its gradient: q [batch, queries, heads, size], k and v [batch, keys, key heads, size]
+    void lower_attention(const Cmd& c) {
+        const bool grad = c.op == OP_ATTENTION_GRAD;
+        Node *q = operand(c, 0), *k = operand(c, 1), *v = operand(c, 2);
+        Node *slopes = operand(c, 3), *docs = operand(c, 4), *prefix = operand(c, 5), *lengths = operand(c, 6);
+        if (q->shape.size() != 4 || k->shape.size() != 4) fail("Attention needs operands [batch, tokens, heads, head size]");
+        const Shape qs = q->shape, ks = k->shape;
+        if (v->shape != ks) fail("Attention: values must have the keys' shape");
+        const int64_t B = qs[0], Tq = qs[1], H = qs[2], D = qs[3], Tk = ks[1], G = ks[2];
+        if (ks[0] != B || ks[3] != D) fail("Attention: queries and keys differ in their batch or head size");
+        if (D < 1 || D > ATTENTION_MAX_DIM) fail("Attention: the head size must lie between 1 and " + std::to_string(ATTENTION_MAX_DIM));
+        if (G < 1 || H < 1 || H % G) fail("Attention: the query heads must be a multiple of the key heads");
+        if (slopes && slopes->shape != Shape{H}) fail("Attention: slopes must be [heads]");
+        if (docs && docs->shape != Shape{B, Tk}) fail("Attention: documents must be [batch, keys]");
+        if (docs && Tq > Tk) fail("Attention: with documents there cannot be more queries than keys");
+        if (prefix && prefix->shape != Shape{B}) fail("Attention: prefix lengths must be [batch]");
+        if (lengths && lengths->shape != Shape{B}) fail("Attention: lengths must be [batch]");
+        if (c.ints[0] != 0 && c.ints[0] != 1) fail("Attention: a flag that is neither 0 nor 1");
+        if (prefix && !c.ints[0]) fail("Attention: a prefix only means something under the causal mask");
+        if (!(c.reals[0] == c.reals[0]) || std::isinf(c.reals[0])) fail("Attention: the scale must be finite");
+        if (!(c.reals[1] >= 0.f) || std::isinf(c.reals[1])) fail("Attention: the cap must be finite and not negative");
+        if (Tq >= (int64_t(1) << 24) || Tk >= (int64_t(1) << 24)) fail("Attention: more than 2^24 tokens");
+        // grids count tiles of 32 tokens of every head in 31 bits
+        if (double(B) * double(H) * double(std::max(Tq, Tk) / 32 + 1) > 2e9) fail("Attention: more than 2^31 tiles");
+        const Shape ls{B, H, Tq};
+        if (grad) {
+            Node *out = operand(c, 7), *lse = operand(c, 8), *dout = operand(c, 9);
+            if (out->shape != qs || dout->shape != qs || lse->shape != ls) fail("AttentionGrad: the output, its gradient or the logarithms have a wrong shape");
+        }
+        if (B * Tq == 0 || Tk == 0) {   // no queries, or nothing to see
+            consume_args(c);
+            bind_result(c, 0, 0.f, qs);
+            if (grad) {
+                bind_result(c, 1, 0.f, ks);
+                bind_result(c, 2, 0.f, ks);
+            } else
+                bind_result(c, 1, -std::numeric_limits<float>::infinity(), ls);
+            return;
+        }
+        const AttentionShape as{B, Tq, Tk, H, G, D};
+        push_oper(c, [&] {
+            std::vector<Access> in;
+            for (size_t i = 0; i < c.args.size(); i++) {
+                Node* n = operand(c, i);
+                const bool flat = (i >= 3 && i <= 6) || i == 8;   // slopes, documents, prefix, lengths; logarithms
+                in.push_back(!n ? Access{} : flat ? flat_operand(n) : operand_access(n));
+            }
+            return in;
+        }, grad ? std::vector<Shape>{qs, ks, ks} : std::vector<Shape>{qs, ls}, {B, Tq, Tk, H, G, D},
+        grad ? attention_grad_workspace(as) : attention_workspace(as, opt_.sm_count));
+    }
+
     void lower_allreduce(const Cmd& c) {
         if (bind_[c.a].kind != Binding::VALUE) fail("AllReduce target '" + name(c.a) + "' must be a tensor, not a view");
         consume(c.a);
@@ -1593,6 +1821,11 @@ class Lowerer {
             if (s.gemm.accumulate) rd.push_back(s.gemm.c);
             if (s.gemm.colvec >= 0) rd.push_back(s.gemm.colvec);
             if (s.gemm.out >= 0) wr.push_back(s.gemm.out);
+            break;
+        case Step::OPER:
+            for (auto& a : s.oper.in) if (a.buf >= 0) rd.push_back(a.buf);
+            for (auto& a : s.oper.out) if (a.buf >= 0) wr.push_back(a.buf);
+            if (s.oper.work >= 0) wr.push_back(s.oper.work);
             break;
         case Step::UPLOAD: wr = {s.buf}; break;
         case Step::ALLREDUCE:
@@ -2899,6 +3132,19 @@ static void dump_block(const Plan& p, const StepBlock& b, int ind, bool src, std
                 o << "\n";
             }
             break;
+        case Step::OPER: {
+            static const char* const names[] = {"rms_norm", "rms_norm_grad", "rotary", "attention", "attention_grad"};
+            o << pad << "#" << s.pos << " " << names[s.oper.op - OP_RMS_NORM];
+            for (auto& a : s.oper.in) o << " " << (a.buf >= 0 ? p.bufs[size_t(a.buf)].name : "-");
+            o << " ->";
+            for (auto& a : s.oper.out) o << " " << (a.buf >= 0 ? p.bufs[size_t(a.buf)].name : "-");
+            o << " [";
+            for (size_t i = 0; i < s.oper.dims.size(); i++) o << (i ? "," : "") << s.oper.dims[i];
+            o << "]";
+            if (s.oper.work >= 0) o << " workspace " << p.bufs[size_t(s.oper.work)].numel * 4 << " B";
+            o << "\n";
+            break;
+        }
         case Step::UPLOAD:
             o << pad << "#" << s.pos << " upload " << p.bufs[s.buf].name << " n=" << s.nelem << "\n";
             break;

@@ -1,0 +1,83 @@
+// Operators of transformer layers: what the lowering has to know about them (shapes, workspaces) and how the runtime
+// launches them.  Host-only declarations; the kernels are in adb_norm.cu, adb_rotary.cu and adb_attention*.cu.
+#pragma once
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+struct CUstream_st;
+
+namespace adb {
+
+// ------------------------------------------------------------------------------------------ root-mean-square norm
+struct NormArgs {
+    const float *x = nullptr, *residual = nullptr, *scale = nullptr;   // residual may be null
+    float *y = nullptr, *h = nullptr;                                  // either may be null; contiguous rows
+    int64_t rows = 0, width = 0, x_rs = 0, r_rs = 0;                   // row strides in elements
+    float eps = 0.f;
+};
+struct NormGradArgs {
+    const float *h = nullptr, *scale = nullptr, *dy = nullptr, *dh = nullptr;   // dh may be null
+    float *dx = nullptr, *dscale = nullptr, *work = nullptr;                    // dx or dscale may be null
+    int64_t rows = 0, width = 0, h_rs = 0, dy_rs = 0, dh_rs = 0;
+    float eps = 0.f;
+    int sm_count = 148;
+};
+constexpr int64_t NORM_GRAD_ONE_PASS = 16384;   // widest row whose share stays in a thread's registers
+// blocks of the gradient kernel: each adds its rows' part of dscale in registers and writes one row of partial sums
+inline int64_t norm_grad_blocks(int64_t rows, int64_t width, int sm_count) {
+    const int64_t rows_per_block = width <= 1024 ? 8 : width <= 2048 ? 2 : 1;
+    const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
+    return std::min<int64_t>(blocks, int64_t(sm_count) * (width <= 4096 ? 2 : 1));
+}
+inline int64_t norm_grad_workspace(int64_t rows, int64_t width, int sm_count) {
+    if (width > NORM_GRAD_ONE_PASS) return rows + width * std::min<int64_t>(rows, 64);
+    return norm_grad_blocks(rows, width, sm_count) * width;
+}
+
+// ------------------------------------------------------------------------------------------ rotary positions
+constexpr int64_t ROTARY_MAX_PAIRS = 4096;   // a block keeps a token's sines and cosines in shared memory
+struct RotaryArgs {
+    const float *x = nullptr, *table = nullptr, *positions = nullptr;   // positions may be null: offset + token
+    float* y = nullptr;                                                 // contiguous
+    int64_t batch = 0, tokens = 0, heads = 0, dim = 0, pairs = 0;
+    int64_t x_bs = 0, x_ts = 0, x_hs = 0, p_bs = 0, p_ts = 0;
+    int64_t offset = 0;
+    int interleaved = 0, inverse = 0;
+    float gain = 1.f;
+    int sm_count = 148;
+};
+
+// ------------------------------------------------------------------------------------------ attention
+constexpr int64_t ATTENTION_MAX_DIM = 256;
+struct AttentionShape {
+    int64_t batch = 0, tq = 0, tk = 0, heads = 0, kv_heads = 0, dim = 0;
+};
+struct Strided4 {   // [batch, tokens, heads, dim], dim contiguous
+    const float* p = nullptr;
+    int64_t bs = 0, ts = 0, hs = 0;
+};
+struct AttentionArgs {
+    AttentionShape s;
+    Strided4 q, k, v, out, dout;            // out (as an operand) and dout: gradient only
+    const float *slopes = nullptr, *docs = nullptr, *prefix = nullptr, *lengths = nullptr;   // each may be null
+    float *o = nullptr, *lse = nullptr;     // forward results (contiguous; lse in base 2; either may be null)
+    const float* lse_in = nullptr;
+    float *dq = nullptr, *dk = nullptr, *dv = nullptr;   // gradient results (contiguous; each may be null)
+    float* work = nullptr;
+    int causal = 0;
+    float scale = 1.f, cap = 0.f;
+    int sm_count = 148;
+};
+inline int64_t attention_workspace(const AttentionShape&, int) { return 0; }
+// one number per query: the gradient of the output times the output
+inline int64_t attention_grad_workspace(const AttentionShape& s) { return s.batch * s.heads * s.tq; }
+
+// Each enqueues its kernels on `stream` and returns how many, or -1 with `err` set.
+int rms_norm_launch(const NormArgs& a, CUstream_st* stream, std::string& err);
+int rms_norm_grad_launch(const NormGradArgs& a, CUstream_st* stream, std::string& err);
+int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err);
+int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+
+}  // namespace adb

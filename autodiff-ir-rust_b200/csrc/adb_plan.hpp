@@ -5,6 +5,7 @@
 //           of outputs (covers Unary / Binary / Movement / ElwExpr of the reference)
 //   REDUCE  row sum with the producing expression fused in front (Reduce / ReduceElwExpr)
 //   GEMM    C = A.B on strided 2-d operands (DotProd)
+//   OPER    an operator of a transformer layer with hand-written kernels (adb_oper.hpp)
 // plus uploads, collectives and host-driven control flow (While / If / EX).
 #pragma once
 #include <climits>
@@ -13,6 +14,7 @@
 #include <vector>
 
 #include "adb_node.hpp"
+#include "adb_oper.hpp"
 
 namespace adb {
 
@@ -104,7 +106,7 @@ struct StepBlock;
 constexpr int64_t DOT_CHUNK_K = 1024;
 
 struct Step {
-    enum Kind { ELW, REDUCE, GEMM, UPLOAD, ALLREDUCE, WHILE, IF, EXIT } kind = EXIT;
+    enum Kind { ELW, REDUCE, GEMM, UPLOAD, ALLREDUCE, WHILE, IF, EXIT, OPER } kind = EXIT;
     int pos = 0;
     int kernel = -1;
     // GEMM: C[M,N] = A[M,K] . B[K,N], strides in elements
@@ -141,6 +143,19 @@ struct Step {
         int64_t colvec_off = 0;
         std::vector<EpiOp> ops;
     } gemm;
+    // OPER: operands and results in the command's order (buf -1: absent, or a result that nothing needs)
+    struct Oper {
+        struct Access {
+            int buf = -1;
+            int64_t off = 0;
+            std::vector<int64_t> stride;   // elements, outermost axis first; empty: one contiguous run
+        };
+        uint8_t op = 0;
+        std::vector<Access> in, out;
+        std::vector<int64_t> dims, ints;
+        std::vector<float> reals;
+        int work = -1;
+    } oper;
     // UPLOAD: payload slot -> buffer; ALLREDUCE: buffer range
     // (a bucketed ALLREDUCE covers `buf` and `more_bufs`, which the arena keeps side by side in that order: one
     // collective over [start of buf, end of the last member))

@@ -417,6 +417,13 @@ class Executor {
             tc_ += d_->gemm.tc_total - tc0;
             break;
         }
+        case Step::OPER: {
+            std::string e;
+            const int n = launch_oper(s.oper, e);
+            if (n < 0) throw CudaFail{"operator: " + e};
+            launches_ += uint64_t(n);
+            break;
+        }
         case Step::UPLOAD: {
             const PayloadSlot& p = plan_.payloads[s.payload];
             auto pf = cp_->prefetch.find(&s);
@@ -459,6 +466,69 @@ class Executor {
             break;
         }
         default: break;
+        }
+    }
+
+    // operators of transformer layers (adb_oper.hpp); operands and results in the order of include/adb200.h
+    int launch_oper(const Step::Oper& o, std::string& err) {
+        using Access = Step::Oper::Access;
+        auto in = [&](size_t i) -> const float* { return o.in[i].buf < 0 ? nullptr : buf_ptr(o.in[i].buf, o.in[i].off); };
+        auto out = [&](size_t i) -> float* { return o.out[i].buf < 0 ? nullptr : buf_ptr(o.out[i].buf, o.out[i].off); };
+        auto rows = [&](size_t i) { return o.in[i].buf < 0 ? int64_t(0) : o.in[i].stride[0]; };
+        float* work = o.work < 0 ? nullptr : buf_ptr(o.work);
+        switch (o.op) {
+        case OP_RMS_NORM: {
+            NormArgs a;
+            a.x = in(0); a.scale = in(1); a.residual = in(2);
+            a.y = out(0); a.h = out(1);
+            a.rows = o.dims[0]; a.width = o.dims[1];
+            a.x_rs = rows(0); a.r_rs = rows(2);
+            a.eps = o.reals[0];
+            return rms_norm_launch(a, cur_stream_, err);
+        }
+        case OP_RMS_NORM_GRAD: {
+            NormGradArgs a;
+            a.h = in(0); a.scale = in(1); a.dy = in(2); a.dh = in(3);
+            a.dx = out(0); a.dscale = out(1); a.work = work;
+            a.rows = o.dims[0]; a.width = o.dims[1];
+            a.h_rs = rows(0); a.dy_rs = rows(2); a.dh_rs = rows(3);
+            a.eps = o.reals[0];
+            a.sm_count = d_->sm_count;
+            return rms_norm_grad_launch(a, cur_stream_, err);
+        }
+        case OP_ROTARY: {
+            RotaryArgs a;
+            a.x = in(0); a.table = in(1); a.positions = in(2); a.y = out(0);
+            a.batch = o.dims[0]; a.tokens = o.dims[1]; a.heads = o.dims[2]; a.dim = o.dims[3]; a.pairs = o.dims[4];
+            a.x_bs = o.in[0].stride[0]; a.x_ts = o.in[0].stride[1]; a.x_hs = o.in[0].stride[2];
+            if (a.positions) { a.p_bs = o.in[2].stride[0]; a.p_ts = o.in[2].stride[1]; }
+            a.interleaved = int(o.ints[0]); a.inverse = int(o.ints[1]); a.offset = o.ints[2];
+            a.gain = o.reals[0];
+            a.sm_count = d_->sm_count;
+            return rotary_launch(a, cur_stream_, err);
+        }
+        default: {
+            const bool grad = o.op == OP_ATTENTION_GRAD;
+            auto four = [&](size_t i) {
+                const Access& x = o.in[i];
+                return Strided4{in(i), x.stride[0], x.stride[1], x.stride[2]};
+            };
+            AttentionArgs a;
+            a.s = {o.dims[0], o.dims[1], o.dims[2], o.dims[3], o.dims[4], o.dims[5]};
+            a.q = four(0); a.k = four(1); a.v = four(2);
+            a.slopes = in(3); a.docs = in(4); a.prefix = in(5); a.lengths = in(6);
+            a.causal = int(o.ints[0]);
+            a.scale = o.reals[0]; a.cap = o.reals[1];
+            a.work = work;
+            a.sm_count = d_->sm_count;
+            if (!grad) {
+                a.o = out(0); a.lse = out(1);
+                return attention_launch(a, cur_stream_, err);
+            }
+            a.out = four(7); a.lse_in = in(8); a.dout = four(9);
+            a.dq = out(0); a.dk = out(1); a.dv = out(2);
+            return attention_grad_launch(a, cur_stream_, err);
+        }
         }
     }
 
@@ -528,6 +598,11 @@ class Executor {
             bufs = {s.gemm.a, s.gemm.b, s.gemm.c};
             if (s.gemm.out >= 0) bufs.push_back(s.gemm.out);
             if (s.gemm.colvec >= 0) bufs.push_back(s.gemm.colvec);
+            break;
+        case Step::OPER:
+            for (auto& a : s.oper.in) if (a.buf >= 0) bufs.push_back(a.buf);
+            for (auto& a : s.oper.out) if (a.buf >= 0) bufs.push_back(a.buf);
+            if (s.oper.work >= 0) bufs.push_back(s.oper.work);
             break;
         case Step::UPLOAD: case Step::ALLREDUCE:
             bufs = {s.buf};
@@ -748,7 +823,7 @@ class Executor {
 
     static bool capturable(const Step& s, const Plan& plan) {
         switch (s.kind) {
-        case Step::ELW: case Step::REDUCE: case Step::GEMM: case Step::ALLREDUCE: return true;
+        case Step::ELW: case Step::REDUCE: case Step::GEMM: case Step::ALLREDUCE: case Step::OPER: return true;
         case Step::UPLOAD: return plan.payloads[s.payload].kind == PAYLOAD_DEVICE;
         default: return false;
         }
@@ -1105,7 +1180,8 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
     d->results.clear();
     // small kept tensors sit side by side at the start of the arena: one copy brings all of them back
     float* block = nullptr;
-    if (plan.results_bytes > 0) {
+    const bool leave = (d->flags & ADB_FLAG_DEVICE_RESULTS) != 0;
+    if (plan.results_bytes > 0 && !leave) {
         if (d->result_block_cap < size_t(plan.results_bytes)) {
             if (d->result_block) cudaFreeHost(d->result_block);
             d->result_block = nullptr;
@@ -1125,7 +1201,9 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
             hr.n = size_t(numel(ri.shape));
             hr.dev = ex.buf_ptr(ri.buf, ri.off);
             const BufferInfo& bi = plan.bufs[size_t(ri.buf)];
-            if (block && !bi.external && bi.arena_off >= 0 && bi.arena_off + (ri.off + int64_t(hr.n)) * 4 <= plan.results_bytes) {
+            if (leave) {
+                // copied when adb_get_tensor asks for it
+            } else if (block && !bi.external && bi.arena_off >= 0 && bi.arena_off + (ri.off + int64_t(hr.n)) * 4 <= plan.results_bytes) {
                 hr.host = block + bi.arena_off / 4 + ri.off;   // inside the shared block: not returned to the pool
                 hr.host_cap = 0;
             } else {
@@ -1133,7 +1211,7 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
                 if (hr.n) ck(cudaMemcpyAsync(hr.host, hr.dev, hr.n * 4, cudaMemcpyDeviceToHost, d->stream), "read-back");
                 d->stats.d2h_bytes += hr.n * 4;
             }
-            hr.fetched = true;
+            hr.fetched = !leave;
         }
         d->results.push_back(std::move(hr));
     }
@@ -1333,6 +1411,20 @@ adb_status adb_get_tensor(adb_device* d, const char* id, const float** data, con
     for (auto& r : d->results)
         if (r.id == id) {
             if (!r.valid) return ADB_NONE;
+            if (!r.fetched) {
+                try {
+                    ck(cudaSetDevice(d->ordinal), "cudaSetDevice");
+                    if (!r.host) r.host = pinned_alloc(d, r.n * 4, r.host_cap);
+                    if (r.n) ck(cudaMemcpyAsync(r.host, r.dev, r.n * 4, cudaMemcpyDeviceToHost, d->stream), "read-back");
+                    ck(cudaStreamSynchronize(d->stream), "read-back");
+                } catch (CudaFail& f) {
+                    d->err = f.msg;
+                    cudaGetLastError();
+                    return ADB_ERR_CUDA;
+                }
+                d->stats.d2h_bytes += uint64_t(r.n) * 4;
+                r.fetched = true;
+            }
             if (data) *data = r.host;
             if (dims) *dims = r.dims.data();
             if (ndim) *ndim = uint32_t(r.dims.size());

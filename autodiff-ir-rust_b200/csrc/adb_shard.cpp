@@ -65,8 +65,11 @@ struct Sharder {
     [[noreturn]] void fail(const std::string& m) { throw IrError("data-parallel rewrite: " + m); }
     const std::string& name(uint32_t id) { return prog.ids[id]; }
 
-    static void reads(const Cmd& c, uint32_t out[2], int& n) {
+    static constexpr int MAX_READS = 10;   // the operator with the most operands
+    static void reads(const Cmd& c, uint32_t out[MAX_READS], int& n) {
         n = 0;
+        for (uint32_t a : c.args)
+            if (a != NO_ID) out[n++] = a;
         switch (c.op) {
         case OP_MUL: case OP_ADD: case OP_DOT: case OP_BATCH_DOT: case OP_CONCAT: case OP_MUL_EQ: case OP_ADD_EQ: out[n++] = c.a; out[n++] = c.b; break;
         case OP_EQZ: case OP_GTZ: case OP_LTZ: case OP_SUM: case OP_MAX: case OP_CONTIG: case OP_EXP2: case OP_LOG2: case OP_SIN:
@@ -74,6 +77,11 @@ struct Sharder {
             out[n++] = c.a; break;
         default: break;
         }
+    }
+    bool wanted(const Cmd& c) const {
+        bool any = false;
+        each_result(c, [&](uint32_t id) { any = any || needed[id]; });
+        return any;
     }
     static bool has_result(uint8_t op) { return !(op == OP_WHILE || op == OP_IF || op == OP_EX || op == OP_HEADING); }
 
@@ -97,8 +105,8 @@ struct Sharder {
                 else if (c.op == OP_IF) {
                     for (auto& cb : c.conds) walk(*cb.second);
                     if (c.else_block) walk(*c.else_block);
-                } else if (has_result(c.op) && needed[c.res]) {
-                    uint32_t r[2];
+                } else if (has_result(c.op) && wanted(c)) {
+                    uint32_t r[MAX_READS];
                     int n;
                     reads(c, r, n);
                     for (int k = 0; k < n; k++)
@@ -191,13 +199,15 @@ struct Sharder {
                 out.defs.insert(in.defs.begin(), in.defs.end());
                 continue;
             }
-            if (!has_result(c.op) || !needed[c.res]) continue;
-            uint32_t r[2];
+            if (!has_result(c.op) || !wanted(c)) continue;
+            uint32_t r[MAX_READS];
             int n;
             reads(c, r, n);
             for (int k = 0; k < n; k++) rd(r[k]);
-            out.defs.insert(c.res);
-            defined.insert(c.res);
+            each_result(c, [&](uint32_t id) {
+                out.defs.insert(id);
+                defined.insert(id);
+            });
         }
     }
     std::map<uint32_t, int> total_reads_;
@@ -267,19 +277,21 @@ struct Sharder {
                 out.push_back(std::move(c));
                 continue;
             }
-            if (!has_result(c.op) || !needed[c.res]) {
+            if (!has_result(c.op) || !wanted(c)) {
                 out.push_back(std::move(c));
                 continue;
             }
             step(c, out);
-            uint32_t res = c.res;
+            std::vector<uint32_t> results;
+            each_result(c, [&](uint32_t id) { results.push_back(id); });
             out.push_back(std::move(c));
-            if (is_dep[res] && info[res].tag == T_PART) {
-                // a kept partial value is completed right where it is produced
-                out.push_back(make_allreduce(res));
-                info[res].tag = T_REP;
-                prog.n_cmds++;
-            }
+            for (uint32_t res : results)
+                if (is_dep[res] && info[res].tag == T_PART) {
+                    // a kept partial value is completed right where it is produced
+                    out.push_back(make_allreduce(res));
+                    info[res].tag = T_REP;
+                    prog.n_cmds++;
+                }
         }
         b.cmds = std::move(out);
     }
@@ -290,11 +302,48 @@ struct Sharder {
         return p;
     }
 
+    // Rows, tokens and sequences are independent of one another: operands that carry the batch stay cut along axis 0 and
+    // give results cut the same way; what belongs to the network (scales, tables, slopes) is whole on every rank.  The
+    // gradient of a norm's scale is a sum over the batch.
+    void operator_step(Cmd& c, std::vector<Cmd>& out) {
+        static const char* const names[] = {"RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionGrad"};
+        const char* what = names[c.op - OP_RMS_NORM];
+        const bool norm = c.op == OP_RMS_NORM || c.op == OP_RMS_NORM_GRAD, rotary = c.op == OP_ROTARY;
+        for (uint32_t a : c.args)
+            if (a != NO_ID) {
+                if (info[a].tag == T_UNDEF) fail("'" + name(a) + "' is read before it is defined");
+                resolve_partial(a, out);
+            }
+        const Info x = info[c.args[0]];
+        const bool cut = x.tag == T_SHARD;
+        if (cut && (x.axis != 0 || (norm && x.dims.size() < 2))) fail(std::string(what) + " of '" + name(c.args[0]) + "' would have to be split along something other than its rows");
+        for (size_t i = 0; i < c.args.size(); i++) {
+            if (c.args[i] == NO_ID) continue;
+            const Info& a = info[c.args[i]];
+            const bool network = ((norm || rotary) && i == 1) || (c.op >= OP_ATTENTION && i == 3) || (rotary && i == 2 && a.dims.size() == 1);
+            const bool is_cut = a.tag == T_SHARD || (a.tag == T_CONST && a.ldims != a.dims);
+            if (network ? is_cut : is_cut != cut) {
+                if (is_cut && a.origin >= 0) redecide(a, -1, std::string(what) + " operand is a broadcast along the batch");
+                if (!is_cut && !network && a.tag == T_CONST) redecide(a, 0, std::string(what) + " operand is a constant along the batch");
+                fail(std::string(what) + ": operand '" + name(c.args[i]) + "' is distributed differently from '" + name(c.args[0]) + "'");
+            }
+            if (!network && is_cut && a.axis != 0) fail(std::string(what) + ": operand '" + name(c.args[i]) + "' is split along an axis other than the batch");
+        }
+        const Tag t = cut ? T_SHARD : T_REP;
+        std::vector<std::vector<int64_t>> dims(c.outs.size(), x.dims);
+        if (c.op == OP_RMS_NORM_GRAD) dims[1] = info[c.args[1]].dims;
+        if (c.op == OP_ATTENTION && x.dims.size() == 4) dims[1] = {x.dims[0], x.dims[2], x.dims[1]};
+        if (c.op == OP_ATTENTION_GRAD) dims[1] = dims[2] = info[c.args[1]].dims;
+        for (size_t k = 0; k < c.outs.size(); k++)
+            if (c.op == OP_RMS_NORM_GRAD && k == 1) set(c.outs[k], cut ? T_PART : T_REP, 0, dims[k], c);
+            else set(c.outs[k], t, 0, dims[k], c);
+    }
+
     void step(Cmd& c, std::vector<Cmd>& out) {
         const int ord = ordinal_++;
         {
             // the result inherits the guess behind the operand that fixes its distribution
-            uint32_t r[2];
+            uint32_t r[MAX_READS];
             int n;
             reads(c, r, n);
             pending_origin_ = -1;
@@ -306,7 +355,7 @@ struct Sharder {
             const bool elementwise = c.op == OP_MUL || c.op == OP_ADD || c.op == OP_MUL_EQ || c.op == OP_ADD_EQ || c.op == OP_EQZ ||
                                      c.op == OP_GTZ || c.op == OP_LTZ || c.op == OP_EXP2 || c.op == OP_LOG2 || c.op == OP_SIN ||
                                      c.op == OP_RECIP || c.op == OP_SQRT || c.op == OP_CONTIG;
-            if (!elementwise)
+            if (!elementwise && !is_operator(c.op))
                 for (int k = 0; k < n; k++) {
                     const Info& x = info[r[k]];
                     if (x.tag == T_CONST && x.ldims != x.dims) redecide(x, -1, "constant '" + name(r[k]) + "' is reshaped after it was cut along the batch");
@@ -466,6 +515,8 @@ struct Sharder {
             else fail("BatchDot of '" + name(c.a) + "' and '" + name(c.b) + "' cannot be split over the batch");
             return;
         }
+        case OP_RMS_NORM: case OP_RMS_NORM_GRAD: case OP_ROTARY: case OP_ATTENTION: case OP_ATTENTION_GRAD:
+            return operator_step(c, out);
         case OP_VIEW: {
             Info a = info[c.a];
             std::vector<int64_t> g = c.dims;

@@ -40,7 +40,12 @@ OPC = {
     # extension: batched matrix product [B, M, K] x [B, K, N] -> [B, M, N] (the reference lists it as missing,
     # TODO.md:22; its attention runs one 2-d DotProduct per head, src/nn/transformer.rs:10-18)
     "BatchDot": 29,
+    # extensions: operators of transformer layers, (name, operands, results, whole parameters, real parameters) with
+    # None for an absent operand; operands, parameters and meaning in include/adb200.h
+    "RmsNorm": 30, "RmsNormGrad": 31, "Rotary": 32, "Attention": 33, "AttentionGrad": 34,
 }
+NO_ID = 0xFFFFFFFF
+OPERATORS = ("RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionGrad")
 
 PAYLOAD_INLINE = 0   # u64 = byte offset of the data inside the blob
 PAYLOAD_HOST = 1     # u64 = host address of n f32 (borrowed for the duration of execute)
@@ -228,6 +233,20 @@ class _Writer:
             self.u16(len(b)); self.body += b
         elif k == "AllReduce":
             self.u32(self.idx(c[1]))
+        elif k in OPERATORS:
+            _, args, outs, ints, reals = c
+            self.u8(len(args))
+            for a in args:
+                self.u32(NO_ID if a is None else self.idx(a))
+            self.u8(len(outs))
+            for o in outs:
+                self.u32(self.idx(o))
+            self.u8(len(ints))
+            for i in ints:
+                self.body += struct.pack("<q", int(i))
+            self.u8(len(reals))
+            for f in reals:
+                self.f32(f)
         else:
             raise ValueError(f"unknown IR command {k}")
 

@@ -60,6 +60,29 @@ typedef enum adb_status {
  *     27 AllReduce id   (extension, no reference counterpart: in-place sum over all ranks)
  *     28 Max a, res     (extension: row maximum of a 2-d tensor, same shape contract as Sum; the reference's kernel
  *                        layer names ReduceOp::Max, src/kernel/kernel_decl.rs:77, but no IR command reaches it)
+ *     29 BatchDot a b res   (extension: [B,M,K] x [B,K,N] -> [B,M,N])
+ *
+ *   Operators of transformer layers (extensions).  operands := u8 n_args, n_args x u32 (0xffffffff: absent, where
+ *   allowed below in brackets), u8 n_results, n_results x u32 (distinct ids), u8 n_ints, n_ints x i64, u8 n_reals,
+ *   n_reals x f32.  The counts are fixed.  A result that nothing needs is not computed where that saves work.
+ *     30 RmsNorm       x scale [residual] -> y h; reals: eps
+ *                      h = x + residual, y = h / sqrt(mean(h^2) + eps) * scale over the last axis
+ *     31 RmsNormGrad   h scale dy [dh] -> dx dscale; reals: eps       (dx is the residual's gradient too)
+ *     32 Rotary        x[B,T,H,D] table[2,P] [positions [T] or [B,T]] -> y; ints: interleaved, inverse, offset;
+ *                      reals: gain.  The first 2 P elements of every head, taken in pairs (2i, 2i+1) or (i, P+i), are
+ *                      turned by position * (table[0][i] + table[1][i]) whole turns (backwards with `inverse`) and
+ *                      multiplied by gain; without positions token t stands at offset + t.  P <= 4096, |offset| <= 2^24.
+ *     33 Attention     q[B,Tq,H,D] k v[B,Tk,G,D] [slopes [H]] [documents [B,Tk]] [prefix [B]] [lengths [B]]
+ *                      -> out[B,Tq,H,D] lse[B,H,Tq] (base 2); ints: causal; reals: scale, cap (0: none)
+ *                      1 <= D <= 256, H a multiple of G, fewer than 2^24 tokens, Tq <= Tk with documents, prefix only with causal.
+ *                      Query i stands at position p = i + n - Tq, n = the sequence's length (Tk without lengths).
+ *                      score = scale q.k, then cap tanh(score / cap), then - slope |p - j|.  Key j is seen when j < n;
+ *                      causal: j <= p or j < prefix; documents: the numbers at p and j agree and are not negative.
+ *                      Causal or with lengths, a query with p < 0 sees nothing.  A query that sees nothing: out 0, lse -inf.
+ *                      Lengths and prefixes are cut to [0, Tk] and to whole numbers (NaN: 0).
+ *     34 AttentionGrad q k v [slopes] [documents] [prefix] [lengths] out lse dout -> dq dk dv; ints, reals as 33.
+ *                      No gradient flows into slopes, documents, prefixes and lengths.
+ *   Operands are read with the strides of the views they are bound to; one whose last axis is not contiguous is copied.
  */
 #define ADB_IR_MAGIC 0x52494441u
 #define ADB_IR_VERSION 1u
@@ -112,6 +135,10 @@ typedef struct adb_config {
                                          of every 4096: the tensor core truncates when it accumulates, so the error
                                          relative to max|C| drops from 3e-5 to 8e-6 (the contract is 1e-4), at ~9 % of the
                                          dot products' speed */
+
+#define ADB_FLAG_DEVICE_RESULTS 16384u  /* adb_execute leaves the kept tensors in HBM: adb_get_tensor copies one when it is asked for
+                                         it, adb_get_tensor_device as without the flag (by default every kept tensor is
+                                         copied to the host inside adb_execute, as the reference does) */
 
 /* Replaces OpenCL::new (src/devices/opencl/device.rs:41-58) + autodiff::set_device's device slot
  * (src/core/autodiff.rs:82-97).  Fails with ADB_ERR_NO_DEVICE when no GPU is present. */

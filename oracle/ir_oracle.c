@@ -67,6 +67,9 @@ typedef struct {
     uint64_t idx_end;
 } Var;
 
+#define MAX_ARGS 10
+#define NO_ID 0xffffffffu
+
 typedef struct Cmd Cmd;
 typedef struct { Cmd *cmds; uint32_t n; } Proc;
 struct Cmd {
@@ -86,6 +89,10 @@ struct Cmd {
     Proc *cond_blocks;
     int has_else;
     Proc else_block;
+    int n_args, n_outs; /* operators */
+    uint32_t args[MAX_ARGS], outs[3];
+    int64_t ints[3];
+    float reals[2];
     uint32_t pos;       /* textual position (top-level index of the enclosing top-level command) */
 };
 
@@ -170,6 +177,26 @@ static int parse_cmd(Oracle *o, Rd *r, Cmd *c, int depth) {
     case 25: break;
     case 26: { uint16_t n = r16(r); if (r->p + n > r->end) r->bad = 1; else r->p += n; } break;
     case 27: c->a = r32(r); c->res = c->a; break;
+    case 30: case 31: case 32: case 33: case 34: { /* operators: operands, results, whole and real parameters */
+        static const uint8_t want[5][4] = { { 3, 2, 0, 1 }, { 4, 2, 0, 1 }, { 3, 1, 3, 1 }, { 7, 2, 1, 2 }, { 10, 3, 1, 2 } };
+        const uint8_t *w = want[c->op - 30];
+        int ok = r8(r) == w[0];
+        for (int i = 0; ok && i < w[0]; i++) {
+            c->args[i] = r32(r);
+            int optional = (c->op == 30 && i == 2) || (c->op == 31 && i == 3) || (c->op == 32 && i == 2) || (c->op >= 33 && i >= 3 && i <= 6);
+            if (c->args[i] == NO_ID ? !optional : c->args[i] >= o->n_ids) ok = 0;
+        }
+        c->n_args = w[0];
+        ok = ok && r8(r) == w[1];
+        for (int i = 0; ok && i < w[1]; i++) if ((c->outs[i] = r32(r)) >= o->n_ids) ok = 0;
+        c->n_outs = w[1];
+        ok = ok && r8(r) == w[2];
+        for (int i = 0; ok && i < w[2]; i++) c->ints[i] = (int64_t)r64(r);
+        ok = ok && r8(r) == w[3];
+        for (int i = 0; ok && i < w[3]; i++) c->reals[i] = rf32(r);
+        if (!ok) { snprintf(o->err, sizeof o->err, "oracle: malformed operator"); return -1; }
+        break;
+    }
     default:
         snprintf(o->err, sizeof o->err, "oracle: unknown opcode %u", c->op);
         return -1;
@@ -219,6 +246,9 @@ static void scan_uses(Oracle *o, Proc *p, int top, uint32_t outer_pos) {
         case 7: case 8: case 9: case 10: case 12: case 13: case 15: case 16: case 17:
         case 18: case 19: case 20: case 21: case 22: case 27: case 28:
             mark_use(o, c->a, pos); break;
+        case 30: case 31: case 32: case 33: case 34:
+            for (int k = 0; k < c->n_args; k++) if (c->args[k] != NO_ID) mark_use(o, c->args[k], pos);
+            break;
         case 23: mark_use(o, c->a, pos); scan_uses(o, &c->block, 0, pos); break;
         case 24:
             for (uint32_t k = 0; k < c->ncond; k++) { mark_use(o, c->cond_ids[k], pos); scan_uses(o, &c->cond_blocks[k], 0, pos); }
@@ -410,6 +440,190 @@ static void bind_buf(Oracle *o, uint32_t id, float *data, const uint64_t *dims, 
 
 /* ------------------------------------------------------------------ execution */
 static int exec_proc(Oracle *o, Proc *p, int top);
+
+/* Operators of transformer layers (extensions; include/adb200.h says what they compute), straight from their formulas in
+ * double precision; the results are rounded once. */
+static int op_fail(Oracle *o, const char *m) { snprintf(o->err, sizeof o->err, "oracle: %s", m); return -1; }
+
+static int same_dims(const Var *a, const Var *b) {
+    if (a->nd != b->nd) return 0;
+    for (int i = 0; i < a->nd; i++) if (a->dims[i] != b->dims[i]) return 0;
+    return 1;
+}
+static int is_vector(const Var *v, uint64_t n) { return v->nd == 1 && v->dims[0] == n; }
+
+static double clip_count(float x, uint64_t most) { /* NaN and negative numbers: none */
+    double v = x > 0 ? (double)x : 0.0;
+    return floor(v < (double)most ? v : (double)most);
+}
+
+static int exec_attention(Oracle *o, Cmd *c, const Var *v[], float *in[]) {
+    const int grad = c->op == 34, causal = c->ints[0] != 0;
+    const double scale = c->reals[0], cap = c->reals[1];
+    if (v[0]->nd != 4 || v[1]->nd != 4 || !same_dims(v[1], v[2])) return op_fail(o, "Attention operands");
+    const uint64_t B = v[0]->dims[0], Tq = v[0]->dims[1], H = v[0]->dims[2], D = v[0]->dims[3], Tk = v[1]->dims[1], G = v[1]->dims[2];
+    if (v[1]->dims[0] != B || v[1]->dims[3] != D || !G || !H || H % G || !D) return op_fail(o, "Attention shapes");
+    if ((in[3] && !is_vector(v[3], H)) || (in[5] && !is_vector(v[5], B)) || (in[6] && !is_vector(v[6], B)) ||
+        (in[4] && (v[4]->nd != 2 || v[4]->dims[0] != B || v[4]->dims[1] != Tk || Tq > Tk)) || (in[5] && !causal))
+        return op_fail(o, "Attention masks");
+    if (grad && (!same_dims(v[7], v[0]) || !same_dims(v[9], v[0]))) return op_fail(o, "AttentionGrad shapes");
+    const uint64_t nq = B * Tq * H * D, nk = B * Tk * G * D;
+    double *a0 = calloc(nq + 1, 8), *a1 = calloc((grad ? nk : B * H * Tq) + 1, 8), *a2 = calloc((grad ? nk : 0) + 1, 8);
+#pragma omp parallel for schedule(dynamic) collapse(2) if (B * G > 1)
+    for (uint64_t b = 0; b < B; b++)
+        for (uint64_t g = 0; g < G; g++) {
+            double *s = malloc((Tk + 1) * 8), *bend = malloc((Tk + 1) * 8);
+            const double n = in[6] ? clip_count(in[6][b], Tk) : (double)Tk, prefix = in[5] ? clip_count(in[5][b], Tk) : 0.0;
+            for (uint64_t h = g * (H / G); h < (g + 1) * (H / G); h++)
+                for (uint64_t i = 0; i < Tq; i++) {
+                    const double pos = (double)i + n - (double)Tq;
+                    const uint64_t row = ((b * Tq + i) * H + h) * D;
+                    const float *q = in[0] + row, *doc = in[4] ? in[4] + b * Tk : NULL;
+                    const int on = !((causal || in[6]) && pos < 0);
+                    double top = -INFINITY, sum = 0;
+                    for (uint64_t j = 0; j < Tk; j++) {
+                        s[j] = -INFINITY;
+                        if (!on || (double)j >= n || (causal && (double)j > pos && (double)j >= prefix)) continue;
+                        if (doc && !(doc[j] >= 0 && doc[(uint64_t)pos] == doc[j])) continue;
+                        const float *k = in[1] + ((b * Tk + j) * G + g) * D;
+                        double x = 0;
+                        for (uint64_t d = 0; d < D; d++) x += (double)q[d] * k[d];
+                        x *= scale;
+                        bend[j] = 1;
+                        if (cap > 0) { double t = tanh(x / cap); x = cap * t; bend[j] = 1 - t * t; }
+                        if (in[3]) x -= (double)in[3][h] * fabs(pos - (double)j);
+                        s[j] = x;
+                        if (x > top) top = x;
+                    }
+                    for (uint64_t j = 0; j < Tk; j++) if (s[j] > -INFINITY) sum += exp(s[j] - top);
+                    if (!grad) a1[(b * H + h) * Tq + i] = sum > 0 ? (top + log(sum)) / log(2.0) : -INFINITY;
+                    if (!(sum > 0)) continue;
+                    double along = 0;
+                    if (grad) for (uint64_t d = 0; d < D; d++) along += (double)in[7][row + d] * in[9][row + d];
+                    for (uint64_t j = 0; j < Tk; j++) {
+                        if (!(s[j] > -INFINITY)) continue;
+                        const double p = exp(s[j] - top) / sum;
+                        const uint64_t at = ((b * Tk + j) * G + g) * D;
+                        if (!grad) { for (uint64_t d = 0; d < D; d++) a0[row + d] += p * in[2][at + d]; continue; }
+                        double dp = 0;
+                        for (uint64_t d = 0; d < D; d++) dp += (double)in[9][row + d] * in[2][at + d];
+                        const double ds = p * (dp - along) * bend[j] * scale;
+                        for (uint64_t d = 0; d < D; d++) {
+                            a0[row + d] += ds * in[1][at + d];
+                            a1[at + d] += ds * q[d];
+                            a2[at + d] += p * in[9][row + d];
+                        }
+                    }
+                }
+            free(s); free(bend);
+        }
+    const uint64_t size[3] = { nq, grad ? nk : B * H * Tq, nk };
+    double *src[3] = { a0, a1, a2 };
+    const uint64_t ld[3] = { B, H, Tq };
+    uint64_t dims[3][MAXD];
+    memcpy(dims[0], v[0]->dims, sizeof dims[0]);
+    memcpy(dims[1], v[1]->dims, sizeof dims[1]);
+    memcpy(dims[2], v[1]->dims, sizeof dims[2]);
+    for (int k = 0; k < c->n_outs; k++) {
+        float *r = pool_alloc(size[k]);
+        for (uint64_t i = 0; i < size[k]; i++) r[i] = (float)src[k][i];
+        if (!grad && k == 1) bind_buf(o, c->outs[k], r, ld, 3);
+        else bind_buf(o, c->outs[k], r, dims[k], 4);
+    }
+    free(a0); free(a1); free(a2);
+    return 0;
+}
+
+static int exec_norm(Oracle *o, Cmd *c, const Var *v[], float *in[]) {
+    const int grad = c->op == 31;
+    if (v[0]->nd < 1 || !v[0]->dims[v[0]->nd - 1]) return op_fail(o, "RmsNorm operand");
+    const uint64_t W = v[0]->dims[v[0]->nd - 1];
+    uint64_t R = 1, dims[MAXD];
+    const int nd = v[0]->nd;
+    for (int i = 0; i < nd - 1; i++) R *= v[0]->dims[i];
+    memcpy(dims, v[0]->dims, sizeof dims);
+    if (!is_vector(v[1], W) || (in[2] && !same_dims(v[2], v[0])) || (grad && in[3] && !same_dims(v[3], v[0]))) return op_fail(o, "RmsNorm shapes");
+    float *r0 = pool_alloc(R * W), *r1 = pool_alloc(grad ? W : R * W);
+    double *dg = calloc(W, 8), *h = malloc(W * 8);
+    for (uint64_t r = 0; r < R; r++) {
+        double s = 0, along = 0;
+        for (uint64_t d = 0; d < W; d++) {
+            h[d] = in[0][r * W + d];
+            if (!grad && in[2]) h[d] += in[2][r * W + d];
+            s += h[d] * h[d];
+        }
+        const double inv = 1 / sqrt(s / (double)W + (double)c->reals[0]);
+        if (!grad) {
+            for (uint64_t d = 0; d < W; d++) { r0[r * W + d] = (float)(h[d] * inv * in[1][d]); r1[r * W + d] = (float)h[d]; }
+            continue;
+        }
+        for (uint64_t d = 0; d < W; d++) along += (double)in[2][r * W + d] * in[1][d] * h[d] * inv;
+        along /= (double)W;
+        for (uint64_t d = 0; d < W; d++) {
+            const double n = h[d] * inv, dy = in[2][r * W + d];
+            dg[d] += dy * n;
+            r0[r * W + d] = (float)((in[3] ? (double)in[3][r * W + d] : 0.0) + inv * (dy * in[1][d] - n * along));
+        }
+    }
+    if (grad) for (uint64_t d = 0; d < W; d++) r1[d] = (float)dg[d];
+    free(dg); free(h);
+    bind_buf(o, c->outs[0], r0, dims, nd);
+    bind_buf(o, c->outs[1], r1, grad ? &W : dims, grad ? 1 : nd);
+    return 0;
+}
+
+static int exec_rotary(Oracle *o, Cmd *c, const Var *v[], float *in[]) {
+    if (v[0]->nd != 4 || v[1]->nd != 2 || v[1]->dims[0] != 2) return op_fail(o, "Rotary operands");
+    const uint64_t B = v[0]->dims[0], T = v[0]->dims[1], H = v[0]->dims[2], D = v[0]->dims[3], P = v[1]->dims[1];
+    uint64_t dims[MAXD];
+    memcpy(dims, v[0]->dims, sizeof dims);
+    if (P < 1 || 2 * P > D) return op_fail(o, "Rotary table");
+    if (in[2] && !is_vector(v[2], T) && !(v[2]->nd == 2 && v[2]->dims[0] == B && v[2]->dims[1] == T)) return op_fail(o, "Rotary positions");
+    float *out = pool_alloc(B * T * H * D);
+    for (uint64_t b = 0; b < B; b++)
+        for (uint64_t t = 0; t < T; t++) {
+            const double pos = in[2] ? in[2][v[2]->nd == 2 ? b * T + t : t] : (double)c->ints[2] + (double)t;
+            for (uint64_t h = 0; h < H; h++) {
+                const uint64_t at = ((b * T + t) * H + h) * D;
+                memcpy(out + at, in[0] + at, D * 4);
+                for (uint64_t p = 0; p < P; p++) {
+                    double turns = pos * ((double)in[1][p] + (double)in[1][P + p]);
+                    const double x = 2 * 3.14159265358979323846 * (turns - floor(turns)), g = c->reals[0];
+                    const double cs = cos(x), sn = c->ints[1] ? -sin(x) : sin(x);
+                    const uint64_t i = at + (c->ints[0] ? 2 * p : p), j = at + (c->ints[0] ? 2 * p + 1 : P + p);
+                    out[i] = (float)(g * (in[0][i] * cs - in[0][j] * sn));
+                    out[j] = (float)(g * (in[0][j] * cs + in[0][i] * sn));
+                }
+            }
+        }
+    bind_buf(o, c->outs[0], out, dims, 4);
+    return 0;
+}
+
+static int exec_operator(Oracle *o, Cmd *c) {
+    const Var *v[MAX_ARGS] = { 0 };
+    float *in[MAX_ARGS] = { 0 };
+    int own[MAX_ARGS] = { 0 };
+    for (int i = 0; i < c->n_args; i++)
+        if (c->args[i] != NO_ID && check_defined(o, c->args[i])) return -1;
+    /* a result may replace an operand: keep what the operands look like */
+    Var *copy = calloc(MAX_ARGS, sizeof(Var));
+    for (int i = 0; i < c->n_args; i++)
+        if (c->args[i] != NO_ID) {
+            copy[i] = o->vars[c->args[i]];
+            v[i] = &copy[i];
+            uint64_t n = 1;
+            for (int d = 0; d < copy[i].nd; d++) n *= copy[i].dims[d];
+            float *m = materialize(o, c->args[i], &own[i]);
+            in[i] = malloc((n + 1) * 4);
+            memcpy(in[i], m, n * 4);
+            if (own[i]) pool_free(m);
+        }
+    int rc = c->op <= 31 ? exec_norm(o, c, v, in) : c->op == 32 ? exec_rotary(o, c, v, in) : exec_attention(o, c, v, in);
+    for (int i = 0; i < c->n_args; i++) free(in[i]);
+    free(copy);
+    return rc;
+}
 
 static int exec_cmd(Oracle *o, Cmd *c) {
     Var *V = o->vars;
@@ -616,6 +830,7 @@ static int exec_cmd(Oracle *o, Cmd *c) {
         bind_buf(o, c->res, out, dims, 3);
         return 0;
     }
+    case 30: case 31: case 32: case 33: case 34: return exec_operator(o, c);
     case 12: case 13: case 15: case 16: { /* aliases */
         if (check_defined(o, c->a)) return -1;
         Var nv; memset(&nv, 0, sizeof nv);
