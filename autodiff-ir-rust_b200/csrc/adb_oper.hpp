@@ -65,11 +65,25 @@ struct AttentionArgs {
     const float* lse_in = nullptr;
     float *dq = nullptr, *dk = nullptr, *dv = nullptr;   // gradient results (contiguous; each may be null)
     float* work = nullptr;
+    int* status = nullptr;   // device word in which a kernel records that a bounded wait ran out
     int causal = 0;
     float scale = 1.f, cap = 0.f;
     int sm_count = 148;
 };
-inline int64_t attention_workspace(const AttentionShape&, int) { return 0; }
+// The tensor-core kernels (adb_attention_tc.cu) take heads of up to 128 elements, padded to panels of 64, and tiles of
+// 128 tokens.
+constexpr int64_t ATTENTION_TC_MAX_DIM = 128, ATTENTION_TC_TILE = 128;
+constexpr int ATTENTION_GAVE_UP = 33;   // first code of a bounded wait of theirs that ran out
+inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
+inline bool attention_uses_tc(const AttentionShape& s) {
+    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 64 && s.tk >= 64 && s.batch * s.kv_heads <= 65535;
+}
+inline int64_t attention_workspace(const AttentionShape& s, int) {
+    if (!attention_uses_tc(s)) return 0;
+    // images of keys and values, a scale for each, document numbers; each part begins on a 256-byte boundary
+    const int64_t tiles = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, n = s.batch * s.kv_heads * tiles;
+    return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64;
+}
 // one number per query: the gradient of the output times the output
 inline int64_t attention_grad_workspace(const AttentionShape& s) { return s.batch * s.heads * s.tq; }
 
@@ -79,5 +93,6 @@ int rms_norm_grad_launch(const NormGradArgs& a, CUstream_st* stream, std::string
 int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err);
 int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);   // where attention_uses_tc
 
 }  // namespace adb

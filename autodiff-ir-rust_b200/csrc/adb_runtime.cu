@@ -91,7 +91,7 @@ static NcclApi g_nccl;
 struct GraphSeg {
     size_t begin = 0, end = 0;       // [begin, end) steps of the block
     cudaGraphExec_t exec = nullptr;  // null: run the steps one by one
-    uint64_t launches = 0, gemms = 0, tc = 0;
+    uint64_t launches = 0, gemms = 0, tc = 0, oper_tc = 0;
 };
 
 // Double-buffered staging for a host payload that a loop body uploads every iteration: the copy for
@@ -520,7 +520,9 @@ class Executor {
             a.causal = int(o.ints[0]);
             a.scale = o.reals[0]; a.cap = o.reals[1];
             a.work = work;
+            a.status = d_->gemm.status;
             a.sm_count = d_->sm_count;
+            if (attention_uses_tc(a.s)) oper_tc_++;
             if (!grad) {
                 a.o = out(0); a.lse = out(1);
                 return attention_launch(a, cur_stream_, err);
@@ -842,7 +844,7 @@ class Executor {
                 GraphSeg g;
                 g.begin = i;
                 g.end = j;
-                uint64_t l0 = launches_, g0 = gemms_, t0 = tc_;
+                uint64_t l0 = launches_, g0 = gemms_, t0 = tc_, o0 = oper_tc_;
                 cudaGraph_t graph = nullptr;
                 ck(cudaStreamBeginCapture(d_->stream, cudaStreamCaptureModeThreadLocal), "begin capture");
                 capturing_ = true;
@@ -862,9 +864,11 @@ class Executor {
                 g.launches = launches_ - l0;
                 g.gemms = gemms_ - g0;
                 g.tc = tc_ - t0;
+                g.oper_tc = oper_tc_ - o0;
                 launches_ = l0;
                 gemms_ = g0;
                 tc_ = t0;
+                oper_tc_ = o0;
                 ck(cudaGraphInstantiate(&g.exec, graph, 0), "graph instantiate");
                 cudaGraphDestroy(graph);
                 segs.push_back(g);
@@ -891,6 +895,7 @@ class Executor {
                     launches_ += g.launches;
                     gemms_ += g.gemms;
                     tc_ += g.tc;
+                    oper_tc_ += g.oper_tc;
                     d_->stats.graph_replays++;
                 } else {
                     run_plain(blk, g.begin, g.end, in_loop);
@@ -973,7 +978,7 @@ class Executor {
 
     static constexpr int COMM_SMS = 8;   // SMs left to NCCL while a collective overlaps dot products
     int gemm_reserve_ = 0;
-    uint64_t launches_ = 0, gemms_ = 0, tc_ = 0;
+    uint64_t launches_ = 0, gemms_ = 0, tc_ = 0, oper_tc_ = 0;   // oper_tc_: operators that ran on the tensor cores
     bool capturing_ = false;
     std::vector<cudaEvent_t> lane_events_;   // dependency events of the capture in progress
     void drop_lane_events() {
@@ -1217,9 +1222,9 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
     }
     ck(cudaEventRecord(ev2, d->stream), "event record");
     ck(cudaStreamSynchronize(d->stream), "synchronize");
-    d->gemm.tc_launches = ex.tc_;  // graph replays launch the kernel without passing through gemm_launch
+    d->gemm.tc_launches = ex.tc_ + ex.oper_tc_;  // graph replays launch the kernel without passing through gemm_launch
     if (int gs = gemm_check_status(d->gemm, d->stream)) {
-        d->err = "tensor-core dot product gave up on a bounded wait (code " + std::to_string(gs) + "); results are invalid";
+        d->err = std::string(gs >= ATTENTION_GAVE_UP ? "attention" : "tensor-core dot product") + " gave up on a bounded wait (code " + std::to_string(gs) + "); results are invalid";
         return ADB_ERR_CUDA;
     }
     float ms_run = 0, ms_rb = 0;
