@@ -60,6 +60,7 @@ struct Strided4 {   // [batch, tokens, heads, dim], dim contiguous
 struct AttentionArgs {
     AttentionShape s;
     Strided4 q, k, v, out, dout;            // out (as an operand) and dout: gradient only
+    int out_vec = 0;                        // out can be read 16 bytes at a time
     const float *slopes = nullptr, *docs = nullptr, *prefix = nullptr, *lengths = nullptr;   // each may be null
     float *o = nullptr, *lse = nullptr;     // forward results (contiguous; lse in base 2; either may be null)
     const float* lse_in = nullptr;
@@ -76,7 +77,7 @@ constexpr int64_t ATTENTION_TC_MAX_DIM = 128, ATTENTION_TC_TILE = 128;
 constexpr int ATTENTION_GAVE_UP = 33;   // first code of a bounded wait of theirs that ran out
 inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
 inline bool attention_uses_tc(const AttentionShape& s) {
-    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 64 && s.tk >= 64 && s.batch * s.kv_heads <= 65535;
+    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 64 && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
 inline int64_t attention_workspace(const AttentionShape& s, int) {
     if (!attention_uses_tc(s)) return 0;
@@ -84,8 +85,14 @@ inline int64_t attention_workspace(const AttentionShape& s, int) {
     const int64_t tiles = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, n = s.batch * s.kv_heads * tiles;
     return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64;
 }
-// one number per query: the gradient of the output times the output
-inline int64_t attention_grad_workspace(const AttentionShape& s) { return s.batch * s.heads * s.tq; }
+inline int64_t attention_grad_workspace(const AttentionShape& s) {
+    if (!attention_uses_tc(s)) return s.batch * s.heads * s.tq;   // one number per query: the gradient of the output times the output
+    const int64_t kt = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, qt = (s.tq + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE;
+    const int64_t nk = s.batch * s.kv_heads * kt, nq = s.batch * s.heads * qt;
+    // images of four operands with their scales, two norms, logarithms and deltas in whole tiles, document numbers
+    return 2 * ((nk + nq) * attention_panels(s.dim) * 8192 + nk + nq + 128) + nk + nq + 128 + 2 * (nq * ATTENTION_TC_TILE + 64) +
+           2 * s.batch * (kt + qt) + 128;
+}
 
 // Each enqueues its kernels on `stream` and returns how many, or -1 with `err` set.
 int rms_norm_launch(const NormArgs& a, CUstream_st* stream, std::string& err);
@@ -93,6 +100,8 @@ int rms_norm_grad_launch(const NormGradArgs& a, CUstream_st* stream, std::string
 int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err);
 int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
-int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);   // where attention_uses_tc
+// where attention_uses_tc
+int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 
 }  // namespace adb

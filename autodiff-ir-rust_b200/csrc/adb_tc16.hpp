@@ -78,30 +78,39 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// shared-memory descriptor, 128-byte swizzle; strides in bytes
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)((sbo >> 4) & 0x3FFF) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory descriptor, 128-byte swizzle, strides in bytes.  Its low word (address and leading stride) may be moved by
+// a distance / 16; the high word depends on the layout alone.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFF) >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29;   // groups of 8 rows 1024 bytes apart
+// keeps the compiler from holding descriptors of every step of a product in registers from one product to the next
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
 }
 // fp16 operands, fp32 accumulator, M = 128; the second operand contracted over its rows (MN-major) or its columns
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_rows, int m = 128) {
     return (1u << 4) | (b_rows ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
-// first operand in tensor memory (lane = row, a column holds two neighbouring fp16 values)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// First operand in tensor memory (lane = row, a column holds two neighbouring fp16 values), second in shared memory.
+// An operand made of halves has 16 columns for 16 elements: 8 with the high halves, then 8 with the low ones, so that it can
+// take the place of the 16 fp32 values it was made from.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+        "mov.b64 y, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH) : "memory");
 }
 // both operands in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+        "mov.b64 x, {%1, %5};\n\t"
+        "mov.b64 y, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH) : "memory");
 }
 
 // 32 columns of the warp's 32 lanes; the values may be used after tmem_wait_load
@@ -114,6 +123,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -135,11 +152,17 @@ __device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t&
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-// the power of two that divides a magnitude into [2^14, 2^15); 1 for zero.  Exponents are kept within +-100, so that the
-// factor and its inverse are normal numbers.
+// 16 elements of a row as an operand, in 16 columns
+__device__ __forceinline__ void tmem_store_halves(uint32_t taddr, const float* x, float f) {
+    uint32_t r[16];
+#pragma unroll
+    for (int k = 0; k < 8; k++) halves(x[2 * k] * f, x[2 * k + 1] * f, r[k], r[8 + k]);
+    tmem_store16(taddr, r);
+}
+// The power of two that divides a magnitude into [2^14, 2^15).  Exponents are kept within +-100, so that the factor and its
+// inverse are normal numbers; zero gets the smallest, so that a tile of zeros does not set the unit of a sum over tiles.
 __device__ __forceinline__ float tile_scale(float largest) {
-    if (!(largest > 0.f)) return 1.f;
-    const int e = min(max(int(__float_as_uint(largest) >> 23) - 127 - 14, -100), 100);
+    const int e = min(max(int(__float_as_uint(fmaxf(largest, 0.f)) >> 23) - 127 - 14, -100), 100);
     return __uint_as_float(uint32_t(e + 127) << 23);
 }
 __device__ __forceinline__ float finite_magnitude(float x) {

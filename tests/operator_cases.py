@@ -2,7 +2,10 @@
 
 Tolerances count roundings of u = 2^-24 (fp32, to nearest): a sum of n terms is off by at most n u of the sum of their
 magnitudes, whatever its order; a product on the tensor cores is assembled from halves of 11 bits, which leaves 2^-21 of
-each term, and added with truncation, which leaves at most 2^-23 for each of the 3 D / 16 instructions.
+each term, and added with truncation, which leaves at most 2^-23 for each of the 3 D / 16 instructions.  Halves are fp16: the
+smallest step is 2^-24, so whatever the size of a value, half a step, 2^-25 of the operand's unit, is left.  The unit is
+chosen so that the largest value of a tile lies in [2^14, 2^15): 2^-39 of that value; weights are kept in units of 2^-10:
+2^-35.  FLOOR_* are those, doubled for the second operand of a product.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import numpy as np
 adb = importlib.import_module("autodiff-ir-rust_b200")
 ad, nn = adb.autodiff, adb.nn
 U = 2.0 ** -24
+FLOOR_VALUE, FLOOR_WEIGHT = 2.0 ** -38, 2.0 ** -34
 
 
 def close(name, got, want, tol):
@@ -200,12 +204,13 @@ def attention_reference(c):
     j = np.arange(tk)
     for n in range(b):
         used_k, used_q = see[n].any(0), see[n].any(1)
+        most = {x: np.abs(np.where((used_k if x in "kv" else used_q)[:, None, None], c[x][n].astype(np.float64), 0)).max(initial=0) for x in ("q", "k", "v", "do")}
         for m in range(h):
             at = m // (h // g)
             q, do = (np.where(used_q[:, None], x[n, :, m].astype(np.float64), 0) for x in (c["q"], c["do"]))
             k, v = (np.where(used_k[:, None], x[n, :, at].astype(np.float64), 0) for x in (c["k"], c["v"]))
             s = q @ k.T * scale
-            err = dot * np.abs(scale) * (np.abs(q) @ np.abs(k).T) + 4 * U * np.abs(s)
+            err = dot * np.abs(scale) * (np.abs(q) @ np.abs(k).T) + 4 * U * np.abs(s) + FLOOR_VALUE * d * np.abs(scale) * most["q"] * most["k"]
             bend = np.ones_like(s)
             if c["cap"]:
                 t = np.tanh(s / c["cap"])
@@ -221,19 +226,21 @@ def attention_reference(c):
             # a weight's relative error: its score's, its row's sum's, the exponential's (argument of up to |s - top|)
             rel = 2 * np.where(see[n], err + 4 * U * np.abs(np.where(see[n], s - top, 0)), 0).max(1, initial=0)[:, None] + 16 * U
             res["out"][0][n, :, m] = o
-            res["out"][1][n, :, m] = (rel + sums + 2.0 ** -21) * (p @ np.abs(v))
+            seen = see[n].astype(np.float64)
+            res["out"][1][n, :, m] = (rel + sums + 2.0 ** -21) * (p @ np.abs(v)) + FLOOR_WEIGHT * seen.sum(1, keepdims=True) * most["v"]
             dp = do @ v.T
             delta = (do * o).sum(1, keepdims=True)
-            size = np.abs(do) @ np.abs(v).T + (np.abs(do) * (p @ np.abs(v))).sum(1, keepdims=True)
+            size = FLOOR_VALUE / U * d * most["do"] * most["v"] + np.abs(do) @ np.abs(v).T + (np.abs(do) * (p @ np.abs(v))).sum(1, keepdims=True)
             ds = p * (dp - delta) * bend * scale
             # the bend's own error is at most 4 err / cap <= 4 u-sized terms already in rel when the cap is at least 1
             worst = p * size * np.abs(scale) * (2 * rel + dot + sums + 2.0 ** -20) + (p * size * np.abs(scale) * 4 * err / c["cap"] if c["cap"] else 0)
+            worst = worst + FLOOR_VALUE * seen * np.abs(scale) * 2 * d * most["do"] * most["v"]     # ds in units of its bound
             res["dq"][0][n, :, m] = ds @ k
-            res["dq"][1][n, :, m] = worst @ np.abs(k)
+            res["dq"][1][n, :, m] = worst @ np.abs(k) + FLOOR_VALUE * worst.sum(1, keepdims=True) / U * most["k"]
             res["dk"][0][n, :, at] += ds.T @ q
-            res["dk"][1][n, :, at] += worst.T @ np.abs(q)
+            res["dk"][1][n, :, at] += worst.T @ np.abs(q) + FLOOR_VALUE * worst.sum(0)[:, None] / U * most["q"]
             res["dv"][0][n, :, at] += p.T @ do
-            res["dv"][1][n, :, at] += (p * (rel + sums + 2.0 ** -21)).T @ np.abs(do)
+            res["dv"][1][n, :, at] += (p * (rel + sums + 2.0 ** -21)).T @ np.abs(do) + FLOOR_WEIGHT * seen.sum(0)[:, None] * most["do"]
     return res
 
 
