@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libadb200.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-SOURCES = ["adb_runtime.cu", "adb_gemm.cu", "adb_noalloc.cu", "adb_norm.cu", "adb_rotary.cu", "adb_attention.cu", "adb_attention_tc.cu",
+SOURCES = ["adb_runtime.cu", "adb_gemm.cu", "adb_noalloc.cu", "adb_norm.cu", "adb_rotary.cu", "adb_attention.cu", "adb_attention_tc.cu", "adb_attention_decode.cu",
            "adb_lower.cpp", "adb_codegen.cpp", "adb_shard.cpp"]
 
 

@@ -1,0 +1,243 @@
+// Attention of a few queries against a long cache: the work is reading the keys and values once.
+//
+// The cache is cut into ranges of keys; a block takes one range of one key head with up to 8 of the query rows (tokens and
+// heads) that share it, and a second kernel joins the ranges' maxima, sums and results in the order of the ranges.  Bound
+// by HBM: 8 bytes per key and element; R query rows cost 4 R flops on the 8 bytes, within what the CUDA cores do beside it
+// up to 8 rows.  Eight lanes read a key together (a lane holds every eighth quad of elements), a warp four keys at
+// once and four such steps in flight; each group of eight lanes has a running maximum and sum of its own, and groups,
+// warps and ranges meet only at the end.
+#include <cuda_runtime.h>
+
+#include "adb_attention.hpp"
+
+namespace adb {
+namespace {
+
+constexpr int THREADS = 256, STEP = 4;
+static_assert(ATTENTION_SPLIT_STEP == THREADS / 8 * STEP, "keys a block takes at a time");
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float sum8(float x) {
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    x += __shfl_xor_sync(0xffffffffu, x, 2);
+    return x + __shfl_xor_sync(0xffffffffu, x, 4);
+}
+
+// R rows, heads of up to 32 NV elements.  partial: [rows of the whole problem][ranges][dim + 2]
+template <int R, int NV>
+__global__ void __launch_bounds__(THREADS, 4 * R * NV + 16 * NV <= 80 ? 2 : 1) adb_attention_split(const AttentionArgs a, const int ranges, const int range_keys, float* partial) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ float4 sq[R][NV * 8];
+    __shared__ float sm[WARPS][R], sl[WARPS][R];
+    __shared__ float4 so[WARPS][R][NV * 8];
+    const int dim = int(a.s.dim), heads = int(a.s.heads), kv_heads = int(a.s.kv_heads), group = heads / kv_heads, tq = int(a.s.tq);
+    const int rows = group * tq, chunks = (rows + R - 1) / R;
+    int at = int(blockIdx.x);
+    const int range = at % ranges;
+    at /= ranges;
+    const int chunk = at % chunks, bg = at / chunks, b = bg / kv_heads, g = bg % kv_heads;
+    const Sight sight(a, b);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, l8 = lane % 8, sub = lane / 8;
+
+    for (int e = threadIdx.x; e < R * NV * 32; e += THREADS) {
+        const int r = e / (NV * 32), c = e % (NV * 32), row = chunk * R + r, i = row / group, h = g * group + row % group;
+        const bool used = row < rows && c < dim && sight.query_used(i + sight.shift);
+        reinterpret_cast<float*>(sq[r])[c] = used ? __ldg(a.q.p + b * a.q.bs + int64_t(i) * a.q.ts + h * a.q.hs + c) : 0.f;
+    }
+    __syncthreads();
+    int pos[R];
+    float doc[R], m[R], l[R];
+    bool on[R];
+    float4 acc[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = chunk * R + r;
+        pos[r] = row / group + sight.shift;
+        on[r] = row < rows && sight.query_used(pos[r]);
+        doc[r] = on[r] && sight.docs ? sight.docs[pos[r]] : 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) acc[r][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const float *kp = a.k.p + b * a.k.bs + g * a.k.hs + 4 * l8, *vp = a.v.p + b * a.v.bs + g * a.v.hs + 4 * l8;
+    const int last_pos = tq - 1 + sight.shift;
+    const int end = min(sight.keys_end(last_pos), (range + 1) * range_keys);
+    for (int j0 = range * range_keys + warp * 4 + sub; j0 - sub < end; j0 += THREADS / 8 * STEP) {   // (the warp's lanes stay together)
+        float4 x[STEP][NV];
+        bool use[STEP];
+#pragma unroll
+        for (int u = 0; u < STEP; u++) {
+            const int j = j0 + u * (THREADS / 8);
+            use[u] = j < end && sight.key_used(j);
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+                x[u][v] = use[u] && 4 * l8 + 32 * v < dim ? __ldg(reinterpret_cast<const float4*>(kp + int64_t(j) * a.k.ts + 32 * v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float s[R][STEP];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int u = 0; u < STEP; u++) s[r][u] = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float4 q = sq[r][8 * v + l8];
+#pragma unroll
+                for (int u = 0; u < STEP; u++)
+                    s[r][u] = fmaf(q.w, x[u][v].w, fmaf(q.z, x[u][v].z, fmaf(q.y, x[u][v].y, fmaf(q.x, x[u][v].x, s[r][u]))));
+            }
+#pragma unroll
+        for (int u = 0; u < STEP; u++) {
+            const int j = j0 + u * (THREADS / 8);
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+                x[u][v] = use[u] && 4 * l8 + 32 * v < dim ? __ldg(reinterpret_cast<const float4*>(vp + int64_t(j) * a.v.ts + 32 * v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int row = chunk * R + r;
+            const ScoreOf score(a, g * group + (row < rows ? row % group : 0));
+            float top = m[r];
+#pragma unroll
+            for (int u = 0; u < STEP; u++) {
+                const int j = j0 + u * (THREADS / 8);
+                float bend;
+                const float dot = sum8(s[r][u]);
+                s[r][u] = use[u] && on[r] && sight.sees(pos[r], j, doc[r]) ? score(dot, pos[r], j, bend) : -INFINITY;
+                top = fmaxf(top, s[r][u]);
+            }
+            const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[r] - base);
+            m[r] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < STEP; u++) {
+                s[r][u] = ex2(s[r][u] - base);
+                sum += s[r][u];
+            }
+            l[r] = fmaf(l[r], keep, sum);
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                float4 o = acc[r][v];
+                o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+                for (int u = 0; u < STEP; u++) {
+                    o.x = fmaf(s[r][u], x[u][v].x, o.x);
+                    o.y = fmaf(s[r][u], x[u][v].y, o.y);
+                    o.z = fmaf(s[r][u], x[u][v].z, o.z);
+                    o.w = fmaf(s[r][u], x[u][v].w, o.w);
+                }
+                acc[r][v] = o;
+            }
+        }
+    }
+    // the warp's four groups, then the block's warps
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float keep = ex2(m[r] - (top == -INFINITY ? 0.f : top));
+        float sum = l[r] * keep;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (lane == 0) { sm[warp][r] = top; sl[warp][r] = sum; }
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            float o[4] = {acc[r][v].x * keep, acc[r][v].y * keep, acc[r][v].z * keep, acc[r][v].w * keep};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                o[e] += __shfl_xor_sync(0xffffffffu, o[e], 8);
+                o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
+            }
+            if (sub == 0) so[warp][r][8 * v + l8] = make_float4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * NV * 32; e += THREADS) {
+        const int r = e / (NV * 32), c = e % (NV * 32), row = chunk * R + r;
+        if (row >= rows || c >= dim) continue;
+        float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) top = fmaxf(top, sm[w][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float f = ex2(sm[w][r] - base);
+            sum = fmaf(sl[w][r], f, sum);
+            o = fmaf(reinterpret_cast<const float*>(so[w][r])[c], f, o);
+        }
+        const int i = row / group, h = g * group + row % group;
+        const int64_t out = (int64_t(b) * tq + i) * heads + h;
+        if (ranges > 1) {
+            float* p = partial + (out * ranges + range) * (dim + 2);
+            p[c] = o;
+            if (c == 0) { p[dim] = top; p[dim + 1] = sum; }
+        } else {
+            if (a.o) a.o[out * dim + c] = sum == 0.f ? 0.f : o / sum;
+            if (a.lse && c == 0) a.lse[(int64_t(b) * heads + h) * tq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
+        }
+    }
+}
+
+// one row of the result a block
+__global__ void __launch_bounds__(128) adb_attention_join(const AttentionArgs a, const int ranges, const float* partial) {
+    const int dim = int(a.s.dim);
+    const int64_t row = blockIdx.x;
+    const float* p = partial + row * ranges * (dim + 2);
+    float top = -INFINITY;
+    for (int s = threadIdx.x % 32; s < ranges; s += 32) top = fmaxf(top, p[int64_t(s) * (dim + 2) + dim]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int c = threadIdx.x; c < dim; c += 128) {
+        float sum = 0.f, o = 0.f;
+        for (int s = 0; s < ranges; s++) {
+            const float* x = p + int64_t(s) * (dim + 2);
+            const float f = ex2(x[dim] - base);
+            sum = fmaf(x[dim + 1], f, sum);
+            o = fmaf(x[c], f, o);
+        }
+        if (a.o) a.o[row * dim + c] = sum == 0.f ? 0.f : o / sum;
+        if (a.lse && c == 0) {
+            const int64_t h = row % a.s.heads, bt = row / a.s.heads, b = bt / a.s.tq, t = bt - b * a.s.tq;
+            a.lse[(b * a.s.heads + h) * a.s.tq + t] = sum == 0.f ? -INFINITY : top + log2f(sum);
+        }
+    }
+}
+
+template <int NV>
+void split(const AttentionArgs& a, int rows, int64_t blocks_of_one, int ranges, int keys, CUstream_st* stream) {
+    // the fewest rows that hold them all, at most what registers take
+    constexpr int MOST = NV <= 4 ? 8 : 4;
+    const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : MOST;
+    const unsigned grid = unsigned(blocks_of_one * ((rows + R - 1) / R) * ranges);
+    if (R == 1) adb_attention_split<1, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
+    else if (R == 2) adb_attention_split<2, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
+    else if (R == 4) adb_attention_split<4, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
+    else adb_attention_split<MOST, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
+}
+
+}  // namespace
+
+int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err) {
+    const AttentionShape& s = a.s;
+    const int rows = int(s.heads / s.kv_heads * s.tq), ranges = int(attention_ranges(s, a.sm_count)), keys = int(attention_range_keys(s, a.sm_count));
+    const int64_t blocks = s.batch * s.kv_heads;
+    if (s.dim <= 32) split<1>(a, rows, blocks, ranges, keys, stream);
+    else if (s.dim <= 64) split<2>(a, rows, blocks, ranges, keys, stream);
+    else if (s.dim <= 96) split<3>(a, rows, blocks, ranges, keys, stream);
+    else if (s.dim <= 128) split<4>(a, rows, blocks, ranges, keys, stream);
+    else split<8>(a, rows, blocks, ranges, keys, stream);
+    if (ranges > 1) adb_attention_join<<<unsigned(s.batch * s.tq * s.heads), 128, 0, stream>>>(a, ranges, a.work);
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return ranges > 1 ? 2 : 1;
+    err = cudaGetErrorString(e);
+    return -1;
+}
+
+}  // namespace adb

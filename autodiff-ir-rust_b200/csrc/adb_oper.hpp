@@ -79,8 +79,20 @@ inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
 inline bool attention_uses_tc(const AttentionShape& s) {
     return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 64 && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
-inline int64_t attention_workspace(const AttentionShape& s, int) {
-    if (!attention_uses_tc(s)) return 0;
+// Few queries (adb_attention_decode.cu): the keys are cut into ranges, so that about eight rounds of two blocks per SM
+// have work and a range keeps a block busy for at least one step.
+constexpr int64_t ATTENTION_SPLIT_STEP = 128;
+inline int64_t attention_range_keys(const AttentionShape& s, int sm_count) {
+    const int64_t rows = s.heads / s.kv_heads * s.tq, blocks = s.batch * s.kv_heads * ((rows + 7) / 8);
+    const int64_t keys = (s.tk * blocks + int64_t(sm_count) * 16 - 1) / (int64_t(sm_count) * 16);
+    return (std::max(keys, ATTENTION_SPLIT_STEP) + ATTENTION_SPLIT_STEP - 1) / ATTENTION_SPLIT_STEP * ATTENTION_SPLIT_STEP;
+}
+inline int64_t attention_ranges(const AttentionShape& s, int sm_count) {
+    const int64_t keys = attention_range_keys(s, sm_count);
+    return (s.tk + keys - 1) / keys;
+}
+inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
+    if (!attention_uses_tc(s)) return s.batch * s.tq * s.heads * attention_ranges(s, sm_count) * (s.dim + 2);
     // images of keys and values, a scale for each, document numbers; each part begins on a 256-byte boundary
     const int64_t tiles = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, n = s.batch * s.kv_heads * tiles;
     return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64;
@@ -100,6 +112,8 @@ int rms_norm_grad_launch(const NormGradArgs& a, CUstream_st* stream, std::string
 int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err);
 int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+// few queries; 16-byte accesses to keys and values
+int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 // where attention_uses_tc
 int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
