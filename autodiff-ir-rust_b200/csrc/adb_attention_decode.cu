@@ -3,9 +3,11 @@
 // The cache is cut into ranges of keys; a block takes one range of one key head with up to 8 of the query rows (tokens and
 // heads) that share it, and a second kernel joins the ranges' maxima, sums and results in the order of the ranges.  Bound
 // by HBM: 8 bytes per key and element; R query rows cost 4 R flops on the 8 bytes, within what the CUDA cores do beside it
-// up to 8 rows.  Eight lanes read a key together (a lane holds every eighth quad of elements), a warp four keys at
-// once and four such steps in flight; each group of eight lanes has a running maximum and sum of its own, and groups,
-// warps and ranges meet only at the end.
+// up to 8 rows.  Eight lanes read a key together (a lane holds every eighth quad of elements), a warp four keys at once;
+// each group of eight lanes has a running maximum and sum of its own, and groups, warps and ranges meet only at the end.
+// Loads go to shared memory asynchronously, three steps deep, each thread fetching what it will read itself: no barrier,
+// and up to 128 KiB in flight on every SM (with loads into registers, 64 KiB at best and none while a step is computed, the
+// kernel reached 3.4 TB/s).
 #include <cuda_runtime.h>
 
 #include "adb_attention.hpp"
@@ -13,8 +15,11 @@
 namespace adb {
 namespace {
 
-constexpr int THREADS = 256, STEP = 4;
-static_assert(ATTENTION_SPLIT_STEP == THREADS / 8 * STEP, "keys a block takes at a time");
+constexpr int THREADS = 256, GROUPS = THREADS / 8, STAGES = 3;
+// keys a group takes at a time: a step of the block is 32 KiB (64 for the largest heads)
+__host__ __device__ constexpr int step_keys(int nv) { return nv == 1 ? 4 : nv == 2 ? 2 : 1; }
+__host__ __device__ constexpr int stage_quads(int nv) { return 2 * step_keys(nv) * nv * THREADS; }
+static_assert(ATTENTION_SPLIT_STEP == GROUPS * 4, "keys a block takes at a time, at most");
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -27,13 +32,21 @@ __device__ __forceinline__ float sum8(float x) {
     return x + __shfl_xor_sync(0xffffffffu, x, 4);
 }
 
+// 16 bytes, or zeros
+__device__ __forceinline__ void fetch(float4* dst, const float* src, bool use) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(use ? 16 : 0) : "memory");
+}
+
 // R rows, heads of up to 32 NV elements.  partial: [rows of the whole problem][ranges][dim + 2]
 template <int R, int NV>
-__global__ void __launch_bounds__(THREADS, 4 * R * NV + 16 * NV <= 80 ? 2 : 1) adb_attention_split(const AttentionArgs a, const int ranges, const int range_keys, float* partial) {
-    constexpr int WARPS = THREADS / 32;
+__global__ void __launch_bounds__(THREADS, R * NV <= 16 && NV <= 4 ? 2 : 1) adb_attention_split(const AttentionArgs a, const int ranges, const int range_keys, float* partial) {
+    constexpr int WARPS = THREADS / 32, STEP = step_keys(NV), QUADS = stage_quads(NV);
+    extern __shared__ float4 ring[];                                    // [STAGES][keys, values][STEP][NV][THREADS]
+    float4(*so)[R][NV * 8] = reinterpret_cast<float4(*)[R][NV * 8]>(ring);   // [WARPS], once the loop is over
+    static_assert(WARPS * R * NV * 8 <= STAGES * QUADS, "the warps' results fit into the ring");
     __shared__ float4 sq[R][NV * 8];
     __shared__ float sm[WARPS][R], sl[WARPS][R];
-    __shared__ float4 so[WARPS][R][NV * 8];
     const int dim = int(a.s.dim), heads = int(a.s.heads), kv_heads = int(a.s.kv_heads), group = heads / kv_heads, tq = int(a.s.tq);
     const int rows = group * tq, chunks = (rows + R - 1) / R;
     int at = int(blockIdx.x);
@@ -67,38 +80,53 @@ __global__ void __launch_bounds__(THREADS, 4 * R * NV + 16 * NV <= 80 ? 2 : 1) a
     const float *kp = a.k.p + b * a.k.bs + g * a.k.hs + 4 * l8, *vp = a.v.p + b * a.v.bs + g * a.v.hs + 4 * l8;
     const int last_pos = tq - 1 + sight.shift;
     const int end = min(sight.keys_end(last_pos), (range + 1) * range_keys);
-    for (int j0 = range * range_keys + warp * 4 + sub; j0 - sub < end; j0 += THREADS / 8 * STEP) {   // (the warp's lanes stay together)
-        float4 x[STEP][NV];
+    const int first = range * range_keys + warp * 4 + sub, steps = max(0, (end - range * range_keys + GROUPS * STEP - 1) / (GROUPS * STEP));
+    auto request = [&](int step) {
+        if (step < steps) {
+            float4* to = ring + (step % STAGES) * QUADS + threadIdx.x;
+#pragma unroll
+            for (int u = 0; u < STEP; u++) {
+                const int j = first + (step * STEP + u) * GROUPS;
+                const bool use = j < end && sight.key_used(j);
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    const bool here = use && 4 * l8 + 32 * v < dim;
+                    fetch(to + (u * NV + v) * THREADS, kp + (here ? int64_t(j) * a.k.ts + 32 * v : 0), here);
+                    fetch(to + ((STEP + u) * NV + v) * THREADS, vp + (here ? int64_t(j) * a.v.ts + 32 * v : 0), here);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    request(0);
+    request(1);
+    for (int step = 0; step < steps; step++) {
+        request(step + 2);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        const float4* from = ring + (step % STAGES) * QUADS + threadIdx.x;
+        const int j0 = first + step * STEP * GROUPS;
         bool use[STEP];
 #pragma unroll
-        for (int u = 0; u < STEP; u++) {
-            const int j = j0 + u * (THREADS / 8);
-            use[u] = j < end && sight.key_used(j);
-#pragma unroll
-            for (int v = 0; v < NV; v++)
-                x[u][v] = use[u] && 4 * l8 + 32 * v < dim ? __ldg(reinterpret_cast<const float4*>(kp + int64_t(j) * a.k.ts + 32 * v)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int u = 0; u < STEP; u++) use[u] = j0 + u * GROUPS < end && sight.key_used(j0 + u * GROUPS);
         float s[R][STEP];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int u = 0; u < STEP; u++) s[r][u] = 0.f;
 #pragma unroll
-        for (int v = 0; v < NV; v++)
+        for (int v = 0; v < NV; v++) {
+            float4 x[STEP];
+#pragma unroll
+            for (int u = 0; u < STEP; u++) x[u] = from[(u * NV + v) * THREADS];
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 const float4 q = sq[r][8 * v + l8];
 #pragma unroll
-                for (int u = 0; u < STEP; u++)
-                    s[r][u] = fmaf(q.w, x[u][v].w, fmaf(q.z, x[u][v].z, fmaf(q.y, x[u][v].y, fmaf(q.x, x[u][v].x, s[r][u]))));
+                for (int u = 0; u < STEP; u++) s[r][u] = fmaf(q.w, x[u].w, fmaf(q.z, x[u].z, fmaf(q.y, x[u].y, fmaf(q.x, x[u].x, s[r][u]))));
             }
-#pragma unroll
-        for (int u = 0; u < STEP; u++) {
-            const int j = j0 + u * (THREADS / 8);
-#pragma unroll
-            for (int v = 0; v < NV; v++)
-                x[u][v] = use[u] && 4 * l8 + 32 * v < dim ? __ldg(reinterpret_cast<const float4*>(vp + int64_t(j) * a.v.ts + 32 * v)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        float keep[R];
+        bool rises = false;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int row = chunk * R + r;
@@ -106,13 +134,15 @@ __global__ void __launch_bounds__(THREADS, 4 * R * NV + 16 * NV <= 80 ? 2 : 1) a
             float top = m[r];
 #pragma unroll
             for (int u = 0; u < STEP; u++) {
-                const int j = j0 + u * (THREADS / 8);
+                const int j = j0 + u * GROUPS;
                 float bend;
                 const float dot = sum8(s[r][u]);
                 s[r][u] = use[u] && on[r] && sight.sees(pos[r], j, doc[r]) ? score(dot, pos[r], j, bend) : -INFINITY;
                 top = fmaxf(top, s[r][u]);
             }
-            const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[r] - base);
+            const float base = top == -INFINITY ? 0.f : top;
+            keep[r] = ex2(m[r] - base);
+            rises = rises || top > m[r];
             m[r] = top;
             float sum = 0.f;
 #pragma unroll
@@ -120,22 +150,33 @@ __global__ void __launch_bounds__(THREADS, 4 * R * NV + 16 * NV <= 80 ? 2 : 1) a
                 s[r][u] = ex2(s[r][u] - base);
                 sum += s[r][u];
             }
-            l[r] = fmaf(l[r], keep, sum);
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                float4 o = acc[r][v];
-                o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
-#pragma unroll
-                for (int u = 0; u < STEP; u++) {
-                    o.x = fmaf(s[r][u], x[u][v].x, o.x);
-                    o.y = fmaf(s[r][u], x[u][v].y, o.y);
-                    o.z = fmaf(s[r][u], x[u][v].z, o.z);
-                    o.w = fmaf(s[r][u], x[u][v].w, o.w);
-                }
-                acc[r][v] = o;
-            }
+            l[r] = fmaf(l[r], keep[r], sum);
         }
+        // (a maximum that stays needs no rescaling: every factor is one.  Maxima rise rarely after the first steps.)
+        if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    acc[r][v].x *= keep[r]; acc[r][v].y *= keep[r]; acc[r][v].z *= keep[r]; acc[r][v].w *= keep[r];
+                }
+        }
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+            for (int u = 0; u < STEP; u++) {
+                const float4 x = from[((STEP + u) * NV + v) * THREADS];
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    acc[r][v].x = fmaf(s[r][u], x.x, acc[r][v].x);
+                    acc[r][v].y = fmaf(s[r][u], x.y, acc[r][v].y);
+                    acc[r][v].z = fmaf(s[r][u], x.z, acc[r][v].z);
+                    acc[r][v].w = fmaf(s[r][u], x.w, acc[r][v].w);
+                }
+            }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     // the warp's four groups, then the block's warps
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -210,16 +251,24 @@ __global__ void __launch_bounds__(128) adb_attention_join(const AttentionArgs a,
     }
 }
 
+template <int R, int NV>
+cudaError_t one(const AttentionArgs& a, unsigned grid, int ranges, int keys, CUstream_st* stream) {
+    constexpr int smem = STAGES * stage_quads(NV) * int(sizeof(float4));
+    const cudaError_t e = cudaFuncSetAttribute((const void*)adb_attention_split<R, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    adb_attention_split<R, NV><<<grid, THREADS, smem, stream>>>(a, ranges, keys, a.work);
+    return cudaGetLastError();
+}
 template <int NV>
-void split(const AttentionArgs& a, int rows, int64_t blocks_of_one, int ranges, int keys, CUstream_st* stream) {
+cudaError_t split(const AttentionArgs& a, int rows, int64_t blocks_of_one, int ranges, int keys, CUstream_st* stream) {
     // the fewest rows that hold them all, at most what registers take
     constexpr int MOST = NV <= 4 ? 8 : 4;
     const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : MOST;
     const unsigned grid = unsigned(blocks_of_one * ((rows + R - 1) / R) * ranges);
-    if (R == 1) adb_attention_split<1, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
-    else if (R == 2) adb_attention_split<2, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
-    else if (R == 4) adb_attention_split<4, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
-    else adb_attention_split<MOST, NV><<<grid, THREADS, 0, stream>>>(a, ranges, keys, a.work);
+    return R == 1   ? one<1, NV>(a, grid, ranges, keys, stream)
+           : R == 2 ? one<2, NV>(a, grid, ranges, keys, stream)
+           : R == 4 ? one<4, NV>(a, grid, ranges, keys, stream)
+                    : one<MOST, NV>(a, grid, ranges, keys, stream);
 }
 
 }  // namespace
@@ -228,13 +277,15 @@ int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::str
     const AttentionShape& s = a.s;
     const int rows = int(s.heads / s.kv_heads * s.tq), ranges = int(attention_ranges(s, a.sm_count)), keys = int(attention_range_keys(s, a.sm_count));
     const int64_t blocks = s.batch * s.kv_heads;
-    if (s.dim <= 32) split<1>(a, rows, blocks, ranges, keys, stream);
-    else if (s.dim <= 64) split<2>(a, rows, blocks, ranges, keys, stream);
-    else if (s.dim <= 96) split<3>(a, rows, blocks, ranges, keys, stream);
-    else if (s.dim <= 128) split<4>(a, rows, blocks, ranges, keys, stream);
-    else split<8>(a, rows, blocks, ranges, keys, stream);
-    if (ranges > 1) adb_attention_join<<<unsigned(s.batch * s.tq * s.heads), 128, 0, stream>>>(a, ranges, a.work);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e = s.dim <= 32    ? split<1>(a, rows, blocks, ranges, keys, stream)
+                    : s.dim <= 64  ? split<2>(a, rows, blocks, ranges, keys, stream)
+                    : s.dim <= 96  ? split<3>(a, rows, blocks, ranges, keys, stream)
+                    : s.dim <= 128 ? split<4>(a, rows, blocks, ranges, keys, stream)
+                                   : split<8>(a, rows, blocks, ranges, keys, stream);
+    if (e == cudaSuccess && ranges > 1) {
+        adb_attention_join<<<unsigned(s.batch * s.tq * s.heads), 128, 0, stream>>>(a, ranges, a.work);
+        e = cudaGetLastError();
+    }
     if (e == cudaSuccess) return ranges > 1 ? 2 : 1;
     err = cudaGetErrorString(e);
     return -1;

@@ -1100,10 +1100,13 @@ static int gemm_launch_one(GemmContext& ctx, const GemmArgs& a, cudaStream_t str
     return 1;
 }
 
-int gemm_check_status(GemmContext& ctx, cudaStream_t stream) {
+bool gemm_fetch_status(GemmContext& ctx, cudaStream_t stream) {
+    if (!ctx.status || ctx.tc_launches == 0) return true;
+    return cudaMemcpyAsync(ctx.status_host, ctx.status, sizeof(int), cudaMemcpyDeviceToHost, stream) == cudaSuccess;
+}
+
+int gemm_take_status(GemmContext& ctx, cudaStream_t stream) {
     if (!ctx.status || ctx.tc_launches == 0) return 0;
-    if (cudaMemcpyAsync(ctx.status_host, ctx.status, sizeof(int), cudaMemcpyDeviceToHost, stream) != cudaSuccess) return -1;
-    if (cudaStreamSynchronize(stream) != cudaSuccess) return -1;
     int s = *ctx.status_host;
     if (s != 0) cudaMemsetAsync(ctx.status, 0, sizeof(int), stream);
     ctx.tc_launches = 0;

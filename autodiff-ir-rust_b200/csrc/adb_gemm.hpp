@@ -57,8 +57,9 @@ void gemm_destroy(GemmContext& ctx);
 // Enqueues the product on `stream`; returns the number of kernels launched, or -1 with `err` set.
 int gemm_launch(GemmContext& ctx, const GemmArgs& a, cudaStream_t stream, std::string& err);
 
-// Reads the status word of the tensor-core kernel (0 = fine; otherwise which bounded wait ran out).
-// Synchronises `stream`.  Returns -1 when the status itself could not be read.
-int gemm_check_status(GemmContext& ctx, cudaStream_t stream);
+// Status word of the tensor-core kernels (0 = fine; otherwise which bounded wait ran out): the first call enqueues its
+// read-back when such kernels were launched, the second returns it once the stream has been synchronised.
+bool gemm_fetch_status(GemmContext& ctx, cudaStream_t stream);
+int gemm_take_status(GemmContext& ctx, cudaStream_t stream);
 
 }  // namespace adb

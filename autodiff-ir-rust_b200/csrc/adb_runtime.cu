@@ -1221,9 +1221,10 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
         d->results.push_back(std::move(hr));
     }
     ck(cudaEventRecord(ev2, d->stream), "event record");
-    ck(cudaStreamSynchronize(d->stream), "synchronize");
     d->gemm.tc_launches = ex.tc_ + ex.oper_tc_;  // graph replays launch the kernel without passing through gemm_launch
-    if (int gs = gemm_check_status(d->gemm, d->stream)) {
+    if (!gemm_fetch_status(d->gemm, d->stream)) throw CudaFail{"status read-back failed"};
+    ck(cudaStreamSynchronize(d->stream), "synchronize");
+    if (int gs = gemm_take_status(d->gemm, d->stream)) {
         d->err = std::string(gs >= ATTENTION_GAVE_UP ? "attention" : "tensor-core dot product") + " gave up on a bounded wait (code " + std::to_string(gs) + "); results are invalid";
         return ADB_ERR_CUDA;
     }
