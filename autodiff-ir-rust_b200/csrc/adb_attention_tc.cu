@@ -16,7 +16,10 @@ namespace {
 using namespace tc16;
 
 constexpr int KT = 128;                 // keys of a tile
-constexpr int SOFTMAX_WARPS = 8;
+// Warps that do the arithmetic between the products: PARTS threads a row, each with a share of its columns.  Four of them
+// rather than two (which have registers to spare) hide the latency of tensor memory, exponentials and barriers better.
+constexpr int PARTS = 4;
+constexpr int SOFTMAX_WARPS = 4 * PARTS, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
 constexpr float P_SHIFT = 10.f;         // weights are kept 2^10 times as large: a weight of 2^-24 still has 20 bits
 
@@ -162,9 +165,9 @@ struct Walk {
 
 enum : int { GAVE_UP_Q = ATTENTION_GAVE_UP, GAVE_UP_SLOT, GAVE_UP_DATA, GAVE_UP_S, GAVE_UP_P, GAVE_UP_O_FULL, GAVE_UP_O_EMPTY };
 
-// a thread's half row of a tensor as fp32, zero outside
+// a thread's share of a row as fp32, zero outside
 template <int N>
-__device__ __forceinline__ void load_half_row(const float* p, int c0, int dim, bool on, bool vec, float (&x)[N]) {
+__device__ __forceinline__ void load_row_part(const float* p, int c0, int dim, bool on, bool vec, float (&x)[N]) {
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -209,59 +212,71 @@ __device__ __forceinline__ void store_row_part(float* p, int c0, int dim, bool v
         }
     }
 }
-__device__ __forceinline__ void pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); }
+// the warps that share a quadrant's rows
+__device__ __forceinline__ void row_sync(int quad) { asm volatile("bar.sync %0, %1;" ::"r"(1 + quad), "n"(32 * PARTS) : "memory"); }
+// largest, or sum, of what the row's threads put down
+__device__ __forceinline__ float row_max(const float* cell, int row) {
+    float x = cell[row];
+#pragma unroll
+    for (int p = 1; p < PARTS; p++) x = fmaxf(x, cell[p * ROWS + row]);
+    return x;
+}
+__device__ __forceinline__ float row_sum(const float* cell, int row) {
+    float x = cell[row];
+#pragma unroll
+    for (int p = 1; p < PARTS; p++) x += cell[p * ROWS + row];
+    return x;
+}
 
 // A product as three: the small ones first, so that the truncating additions meet a small sum.
 // First operand in tensor memory, second an image contracted over its columns.
 template <int P, int PANEL>
-__device__ __forceinline__ void scores_mma(uint32_t d, uint32_t a, uint32_t image, uint32_t id) {
-    const uint32_t b = fresh(desc_low(image, 0));
-    a = fresh(a);
+__device__ __forceinline__ void scores_mma(uint32_t e, uint32_t d, uint32_t a, uint32_t image, uint32_t id) {
+    const uint32_t b = desc_low(image, 0);
     constexpr auto at = [](int half, int j) { return uint32_t(half * P * PANEL + (j / 4) * PANEL + (j % 4) * 32) >> 4; };
 #pragma unroll
     for (int j = 0; j < 4 * P; j++) {   // 16 columns each
-        mma_ts(d, a + 16 * j + 8, b + at(0, j), id, j != 0);
-        mma_ts(d, a + 16 * j, b + at(1, j), id, 1);
+        mma_ts(e, d, a + 16 * j + 8, b + at(0, j), id, j != 0);
+        mma_ts(e, d, a + 16 * j, b + at(1, j), id, 1);
     }
 #pragma unroll
-    for (int j = 0; j < 4 * P; j++) mma_ts(d, a + 16 * j, b + at(0, j), id, 1);
+    for (int j = 0; j < 4 * P; j++) mma_ts(e, d, a + 16 * j, b + at(0, j), id, 1);
 }
 // the same with the first operand an image of 128 rows in shared memory
 template <int P, int PANEL>
-__device__ __forceinline__ void scores_mma_ss(uint32_t d, uint32_t own, uint32_t image, uint32_t id) {
-    const uint32_t a = fresh(desc_low(own, 0)), b = fresh(desc_low(image, 0));
+__device__ __forceinline__ void scores_mma_ss(uint32_t e, uint32_t d, uint32_t own, uint32_t image, uint32_t id) {
+    const uint32_t a = desc_low(own, 0), b = desc_low(image, 0);
     constexpr auto at = [](int panel, int half, int j) { return uint32_t(half * P * panel + (j / 4) * panel + (j % 4) * 32) >> 4; };
 #pragma unroll
     for (int j = 0; j < 4 * P; j++) {
-        mma_ss(d, a + at(PANEL_BYTES, 1, j), b + at(PANEL, 0, j), id, j != 0);
-        mma_ss(d, a + at(PANEL_BYTES, 0, j), b + at(PANEL, 1, j), id, 1);
+        mma_ss(e, d, a + at(PANEL_BYTES, 1, j), b + at(PANEL, 0, j), id, j != 0);
+        mma_ss(e, d, a + at(PANEL_BYTES, 0, j), b + at(PANEL, 1, j), id, 1);
     }
 #pragma unroll
-    for (int j = 0; j < 4 * P; j++) mma_ss(d, a + at(PANEL_BYTES, 0, j), b + at(PANEL, 0, j), id, 1);
+    for (int j = 0; j < 4 * P; j++) mma_ss(e, d, a + at(PANEL_BYTES, 0, j), b + at(PANEL, 0, j), id, 1);
 }
 // first operand in tensor memory, second an image contracted over its rows, 16 at a time
 template <int P, int PANEL, int STEPS>
-__device__ __forceinline__ void rows_mma(uint32_t d, uint32_t a, uint32_t image, uint32_t id) {
-    const uint32_t b = fresh(desc_low(image, PANEL));
-    a = fresh(a);
+__device__ __forceinline__ void rows_mma(uint32_t e, uint32_t d, uint32_t a, uint32_t image, uint32_t id) {
+    const uint32_t b = desc_low(image, PANEL);
     constexpr auto at = [](int half, int j) { return uint32_t(half * P * PANEL + j * 2048) >> 4; };
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
-        mma_ts(d, a + 16 * j + 8, b + at(0, j), id, j != 0);
-        mma_ts(d, a + 16 * j, b + at(1, j), id, 1);
+        mma_ts(e, d, a + 16 * j + 8, b + at(0, j), id, j != 0);
+        mma_ts(e, d, a + 16 * j, b + at(1, j), id, 1);
     }
 #pragma unroll
-    for (int j = 0; j < STEPS; j++) mma_ts(d, a + 16 * j, b + at(0, j), id, 1);
+    for (int j = 0; j < STEPS; j++) mma_ts(e, d, a + 16 * j, b + at(0, j), id, 1);
 }
 
 // ------------------------------------------------------------------------------------------ forward
 // A block owns 128 queries of one head; keys and values pass by in tiles of 128.  Roles:
-//   warp 9, one thread   bulk copies of key and value images into a ring of three slots
-//   warp 8, one thread   S = Q K^T (into one of two buffers) and O = P V, in the order S0 S1 O0 S2 O1 ... so that the
-//                        tensor cores work on S(i+1) while the weights of tile i are computed
-//   warps 0-7            two threads a row, half of the columns each: scores out of tensor memory, the running maximum
-//                        (shared between the two through shared memory), weights back as fp16 halves over the scores
-//                        they came from, then O of the tile before added to the result in registers
+//   loading warp, one thread    bulk copies of key and value images into a ring of three slots
+//   issuing warp, one thread    S = Q K^T (into one of two buffers) and O = P V, in the order S0 S1 O0 S2 O1 ... so that the
+//                               tensor cores work on S(i+1) while the weights of tile i are computed
+//   16 warps                    four threads a row, a quarter of the columns each: scores out of tensor memory, the running
+//                               maximum (shared between the four through shared memory), weights back as fp16 halves over
+//                               the scores they came from, then O of the tile before added to the result in registers
 // Q lives in tensor memory (read there, the products fetch only the other operand from shared memory, which would
 // otherwise be the bound), O is drained after every tile: the tensor core truncates as it accumulates, so a sum over a
 // long sequence is kept by rounded adds in registers.  Tensor memory: Q 128 columns, S 2 x 128, O 128.
@@ -279,18 +294,18 @@ struct ForwardShared {
     static constexpr int SLOTS = P == 2 ? 3 : 6;
     static constexpr int SLOT_BYTES = image_bytes(P);
     static constexpr int BARS = 2 * SLOTS + 7;
-    static constexpr int BYTES = 1024 + SLOTS * SLOT_BYTES + 2 * 2 * ROWS * 4 + BARS * 8 + 16 + 16 * 4;
+    static constexpr int BYTES = 1024 + SLOTS * SLOT_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16 + 2 * SOFTMAX_WARPS * 4;
 };
 
 template <int P, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs f) {
     using Shared = ForwardShared<P>;
-    constexpr int SLOTS = Shared::SLOTS, DP = 64 * P, HALF = DP / 2, N_ACC = HALF;
+    constexpr int SLOTS = Shared::SLOTS, DP = 64 * P, SHARE = DP / PARTS, KEYS = KT / PARTS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    float* exchange = reinterpret_cast<float*>(gen + SLOTS * Shared::SLOT_BYTES);   // [2][2][128]
-    const uint32_t bars = base + SLOTS * Shared::SLOT_BYTES + 2 * 2 * ROWS * 4;
+    float* exchange = reinterpret_cast<float*>(gen + SLOTS * Shared::SLOT_BYTES);   // [2][PARTS][128]
+    const uint32_t bars = base + SLOTS * Shared::SLOT_BYTES + 2 * PARTS * ROWS * 4;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (SLOTS + s); };
     auto s_full = [&](int i) { return bars + 8u * (2 * SLOTS + i); };
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (bars - base) + Shared::BARS * 8);
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* doc_span = const_cast<int*>(reinterpret_cast<volatile int*>(tmem_slot + 2));   // [2]
-    volatile int* agreed = reinterpret_cast<volatile int*>(tmem_slot + 4);              // [2][2][4]: tile parity, half, quadrant
+    volatile int* agreed = reinterpret_cast<volatile int*>(tmem_slot + 4);              // [2][SOFTMAX_WARPS]: tile parity, warp
 
     const AttentionArgs& a = f.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -320,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         doc_span[1] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
+    if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
     __syncthreads();
     if (sight.docs && threadIdx.x < ROWS && q0 + int(threadIdx.x) < tq) {
         const int pos = q0 + int(threadIdx.x) + sight.shift;
@@ -342,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     walk.hi = doc_span[1] < 0 ? -1.f : __int_as_float(doc_span[1]);
     const int64_t image0 = (int64_t(b) * kv_heads + g) * k_tiles;
 
-    if (warp == 9) {
+    if (warp == LOAD_WARP) {
         if (lane == 0) {
             uint32_t n = 0;
             auto fetch = [&](const uint8_t* images, int tile) {
@@ -365,169 +380,160 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 for (uint32_t k = n > SLOTS ? n - SLOTS : 0; k < n; k++)
                     for (uint32_t it = 0; it < SPIN_LIMIT && !bar_test(full(k % SLOTS), (k / SLOTS) & 1); it++) __nanosleep(64);
         }
-    } else if (warp == 8) {
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc(KT, false), id_o = idesc(DP, true);
-            uint32_t n = 0;
-            auto slot = [&](uint32_t k) { return base + (k % SLOTS) * Shared::SLOT_BYTES; };
-            auto landed = [&](uint32_t k) { return bar_wait(full(k % SLOTS), (k / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
-            int t = walk.first();
-            bool ok = t < 0 || bar_wait(q_ready, 0, stop, f.status, GAVE_UP_Q);
+    } else if (warp == MMA_WARP) {
+        constexpr uint32_t id_s = idesc(KT, false), id_o = idesc(DP, true);
+        const uint32_t e = elect(), tm = uniform(tmem), from = uniform(base);
+        uint32_t n = 0;
+        auto slot = [&](uint32_t k) { return from + (k % SLOTS) * Shared::SLOT_BYTES; };
+        auto landed = [&](uint32_t k) { return bar_wait_warp(full(k % SLOTS), (k / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
+        int t = uniform(walk.first());
+        bool ok = t < 0 || bar_wait_warp(q_ready, 0, stop, f.status, GAVE_UP_Q);
+        fence_after();
+        auto scores = [&](int i) {
+            if (!landed(n)) return false;
+            scores_mma<P, PANEL_BYTES>(e, tm + 128 + 128 * (i & 1), tm, slot(n), id_s);
+            mma_commit(e, empty(n % SLOTS));
+            mma_commit(e, s_full(i & 1));
+            n++;
+            return true;
+        };
+        if (ok && t >= 0) ok = scores(0);
+        for (int i = 0; ok && t >= 0; i++) {
+            const int next = uniform(walk.from(t + 1));
+            if (next >= 0 && !scores(i + 1)) break;
+            // (waits for O's drain are satisfied at once for the first tile: the barrier's phase before the first)
+            if (!bar_wait_warp(p_ready(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_P) || !bar_wait_warp(o_empty, (i & 1) ^ 1, stop, f.status, GAVE_UP_O_EMPTY) || !landed(n)) break;
             fence_after();
-            auto scores = [&](int i) {
-                if (!landed(n)) return false;
-                scores_mma<P, PANEL_BYTES>(tmem + 128 + 128 * (i & 1), tmem, slot(n), id_s);
-                mma_commit(empty(n % SLOTS));
-                mma_commit(s_full(i & 1));
-                n++;
-                return true;
-            };
-            if (ok && t >= 0) ok = scores(0);
-            for (int i = 0; ok && t >= 0; i++) {
-                const int next = walk.from(t + 1);
-                if (next >= 0 && !scores(i + 1)) break;
-                // (waits for O's drain are satisfied at once for the first tile: the barrier's phase before the first)
-                if (!bar_wait(p_ready(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_P) || !bar_wait(o_empty, (i & 1) ^ 1, stop, f.status, GAVE_UP_O_EMPTY) || !landed(n)) break;
-                fence_after();
-                rows_mma<P, PANEL_BYTES, 8>(tmem + 384, tmem + 128 + 128 * (i & 1), slot(n), id_o);
-                mma_commit(empty(n % SLOTS));
-                mma_commit(o_full);
-                n++;
-                t = next;
-            }
+            rows_mma<P, PANEL_BYTES, 8>(e, tm + 384, tm + 128 + 128 * (i & 1), slot(n), id_o);
+            mma_commit(e, empty(n % SLOTS));
+            mma_commit(e, o_full);
+            n++;
+            t = next;
         }
     } else {
-        const int quad = warp & 3, half = warp >> 2, row = 32 * quad + lane, q = q0 + row, pos = q + sight.shift;
+        const int quad = warp & 3, part = warp >> 2, row = 32 * quad + lane, q = q0 + row, pos = q + sight.shift;
         const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
         const bool on = q < tq && sight.query_used(pos);
         const float doc = on && sight.docs ? sight.docs[pos] : 0.f;
         float q_scale;
         {
-            float x[HALF];
-            load_half_row<HALF>(a.q.p + b * a.q.bs + int64_t(on ? q : 0) * a.q.ts + h * a.q.hs, half * HALF, dim, on, f.q_vec, x);
-            exchange[half * ROWS + row] = largest(x);
-            pair_sync(quad);
-            q_scale = tile_scale(fmaxf(exchange[row], exchange[ROWS + row]));
-            store_halves<HALF>(lanes + half * HALF, x, 1.f / q_scale);
+            float x[SHARE];
+            load_row_part<SHARE>(a.q.p + b * a.q.bs + int64_t(on ? q : 0) * a.q.ts + h * a.q.hs, part * SHARE, dim, on, f.q_vec, x);
+            exchange[part * ROWS + row] = largest(x);
+            row_sync(quad);
+            q_scale = tile_scale(row_max(exchange, row));
+            store_halves<SHARE>(lanes + part * SHARE, x, 1.f / q_scale);
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(q_ready);
-            pair_sync(quad);
+            row_sync(quad);
         }
         const ScoreOf score(a, h);
         const float cap2 = score.cap2, slope2 = score.slope2;
-        float acc[N_ACC], m = -INFINITY, l = 0.f, keep = 0.f, v_before = 0.f;
+        float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_before = 0.f;
 #pragma unroll
-        for (int c = 0; c < N_ACC; c++) acc[c] = 0.f;
+        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
         bool ok = true;
         auto drain = [&](int i) {   // O of tile i
             if (!bar_wait_warp(o_full, i & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
             fence_after();
-#pragma unroll
-            for (int c = 0; c < N_ACC; c += 32) {
-                uint32_t r[32];
-                tmem_load32(lanes + 384 + half * HALF + c, r);
-                tmem_wait_load();
-#pragma unroll
-                for (int k = 0; k < 32; k++) acc[c + k] = fmaf(__uint_as_float(r[k]), v_before, acc[c + k] * keep);
-            }
+            uint32_t r[SHARE];
+            tmem_load(lanes + 384 + part * SHARE, r);
+            tmem_wait_load();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(o_empty);
+#pragma unroll
+            for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), v_before, acc[c] * keep);
             return true;
         };
         int i = 0;
         const int pos_first = q0 + sight.shift;
         for (int t = walk.first(); t >= 0; t = walk.from(t + 1), i++) {
-            const int k0 = t * KT + 64 * half;
+            const int k0 = t * KT + KEYS * part;
             const float mul = q_scale * __ldg(f.k_scale + image0 + t) * score.mul, v_scale = __ldg(f.v_scale + image0 + t);
-            // a warp that gives up still meets its partner once, so that neither waits for the other for good
+            // a warp that gives up still meets the others once, so that none waits for it for good
             ok = ok && bar_wait_warp(s_full(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_S);
             fence_after();
-            const uint32_t at = lanes + 128 + 128 * (i & 1);
-            float s[64];
+            const uint32_t at = lanes + 128 + 128 * (i & 1) + KEYS * part;
+            float s[KEYS];
             {
-                uint32_t r[32];
-                tmem_load32(at + 64 * half, r);
+                uint32_t r[KEYS];
+                tmem_load(at, r);
                 tmem_wait_load();
 #pragma unroll
-                for (int c = 0; c < 32; c++) s[c] = __uint_as_float(r[c]) * mul;
-                tmem_load32(at + 64 * half + 32, r);
-                tmem_wait_load();
-#pragma unroll
-                for (int c = 0; c < 32; c++) s[32 + c] = __uint_as_float(r[c]) * mul;
+                for (int c = 0; c < KEYS; c++) s[c] = __uint_as_float(r[c]) * mul;
             }
             if constexpr (CAP) {
 #pragma unroll
-                for (int c = 0; c < 64; c++) s[c] = cap2 * tanh_exact(s[c]);
+                for (int c = 0; c < KEYS; c++) s[c] = cap2 * tanh_exact(s[c]);
             }
             if constexpr (BIAS) {
                 const float away = float(pos - k0);
 #pragma unroll
-                for (int c = 0; c < 64; c++) s[c] = fmaf(-slope2, fabsf(away - float(c)), s[c]);
+                for (int c = 0; c < KEYS; c++) s[c] = fmaf(-slope2, fabsf(away - float(c)), s[c]);
             }
-            const bool partly = k0 + 63 >= sight.n || sight.docs || (sight.causal && k0 + 63 > pos_first && k0 + 63 >= sight.prefix);
-            if (partly) {
+            const int k_last = k0 + KEYS - 1;
+            if (k_last >= sight.n || sight.docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
                 // keys from `ahead` on are hidden by the length or the order
                 const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
 #pragma unroll
-                for (int c = 0; c < 64; c++)
+                for (int c = 0; c < KEYS; c++)
                     if (c >= ahead || (sight.docs && __ldg(sight.docs + k0 + c) != doc)) s[c] = -INFINITY;
             }
-            float top = s[0];
+            float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 1; c < 64; c++) top = fmaxf(top, s[c]);
-            float* cell = exchange + (i & 1) * 2 * ROWS;
-            cell[half * ROWS + row] = top;
-            if (lane == 0) agreed[8 * (i & 1) + 4 * half + quad] = ok;
-            pair_sync(quad);
-            ok = agreed[8 * (i & 1) + quad] && agreed[8 * (i & 1) + 4 + quad];
+            for (int c = 4; c < KEYS; c++) tops[c & 3] = fmaxf(tops[c & 3], s[c]);
+            float* cell = exchange + (i & 1) * PARTS * ROWS;
+            cell[part * ROWS + row] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            if (lane == 0) agreed[SOFTMAX_WARPS * (i & 1) + warp] = ok;
+            row_sync(quad);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
             if (!ok) break;
-            top = fmaxf(m, fmaxf(cell[row], cell[ROWS + row]));
+            const float top = fmaxf(m, row_max(cell, row));
             const float from = (top == -INFINITY ? 0.f : top) - P_SHIFT;
             const float fade = ex2(m - from - P_SHIFT);
             m = top;
-            float sum0 = 0.f, sum1 = 0.f;
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
+            for (int c = 0; c < KEYS; c++) {
                 s[c] = ex2(s[c] - from);
-                s[c + 1] = ex2(s[c + 1] - from);
-                sum0 += s[c];
-                sum1 += s[c + 1];
+                sums[c & 3] += s[c];
             }
-            store_halves<64>(at + 64 * half, s, 1.f);
+            store_halves<KEYS>(at, s, 1.f);
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_ready(i & 1));
-            l = fmaf(l, fade, sum0 + sum1);
+            l = fmaf(l, fade, (sums[0] + sums[1]) + (sums[2] + sums[3]));
             if (i > 0) ok = drain(i - 1);
             keep = fade;
             v_before = v_scale;
         }
         if (ok && i > 0) ok = drain(i - 1);
-        float* cell = exchange + (i & 1) * 2 * ROWS;   // (the last tile's may still be being read)
-        cell[half * ROWS + row] = l;
-        pair_sync(quad);
+        float* cell = exchange + (i & 1) * PARTS * ROWS;   // (the last tile's may still be being read)
+        cell[part * ROWS + row] = l;
+        row_sync(quad);
         if (ok) {
-            l = cell[row] + cell[ROWS + row];
+            l = row_sum(cell, row);
             if (q < tq) {
                 const bool any = on && l != 0.f;
                 if (a.o) {
                     if (!any)
 #pragma unroll
-                        for (int c = 0; c < N_ACC; c++) acc[c] = 0.f;
-                    store_row_part<N_ACC>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, half * HALF, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
+                        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+                    store_row_part<SHARE>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
                 }
-                if (a.lse && half == 0) a.lse[int64_t(bh) * tq + q] = any ? m + (log2f(l) - P_SHIFT) : -INFINITY;
+                if (a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + (log2f(l) - P_SHIFT) : -INFINITY;
             }
         }
     }
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------------------ gradient
@@ -576,19 +582,19 @@ struct QueryGradShared {
     static constexpr int SLOTS = 3;   // of keys and of values
     static constexpr int SLOT_BYTES = 2 * P * SUB_BYTES;
     static constexpr int BARS = 4 * SLOTS + 7;
-    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + 2 * ROWS * 4 + BARS * 8 + 32;
+    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + PARTS * ROWS * 4 + BARS * 8 + 32;
 };
 
 template <int P, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs f) {
     using Shared = QueryGradShared<P>;
-    constexpr int SLOTS = Shared::SLOTS, SLOT = Shared::SLOT_BYTES, DP = 64 * P, HALF = DP / 2;
+    constexpr int SLOTS = Shared::SLOTS, SLOT = Shared::SLOT_BYTES, DP = 64 * P, SHARE = DP / PARTS, KEYS = GT / PARTS;
     constexpr uint32_t C_Q = 0, C_DO = DP, C_DQ = 2 * DP, C_S = 3 * DP, C_DP = 3 * DP + 64;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    float* exchange = reinterpret_cast<float*>(gen + 2 * SLOTS * SLOT);   // [2][128]
-    const uint32_t bars = base + 2 * SLOTS * SLOT + 2 * ROWS * 4;
+    float* exchange = reinterpret_cast<float*>(gen + 2 * SLOTS * SLOT);   // [PARTS][128]
+    const uint32_t bars = base + 2 * SLOTS * SLOT + PARTS * ROWS * 4;
     auto k_slot = [&](uint32_t n) { return base + (n % SLOTS) * SLOT; };
     auto v_slot = [&](uint32_t n) { return base + (SLOTS + n % SLOTS) * SLOT; };
     auto k_full = [&](uint32_t n) { return bars + 8u * (n % SLOTS); };
@@ -626,7 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         cells[2] = cells[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
+    if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
     __syncthreads();
     block_max(&cells[2], f.k.scale + image0, (keys_end + ROWS - 1) / ROWS);
     block_max(&cells[3], f.v.norm + image0, (keys_end + ROWS - 1) / ROWS);
@@ -645,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         walk.hi = own.y;
     }
 
-    if (warp == 9) {
+    if (warp == LOAD_WARP) {
         if (lane == 0) {
             uint32_t n = 0;
             bool ok = true;
@@ -665,46 +671,47 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                 for (uint32_t k = n > SLOTS ? n - SLOTS : 0; k < n; k++)
                     for (uint32_t it = 0; it < SPIN_LIMIT && !(bar_test(k_full(k), (k / SLOTS) & 1) && bar_test(v_full(k), (k / SLOTS) & 1)); it++) __nanosleep(64);
         }
-    } else if (warp == 8) {
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc(GT, false), id_acc = idesc(DP, true);
-            auto landed = [&](uint32_t bar, uint32_t n) { return bar_wait(bar, (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
-            auto s_product = [&](uint32_t n) {
-                if (!landed(k_full(n), n)) return false;
-                scores_mma<P, SUB_BYTES>(tmem + C_S, tmem + C_Q, k_slot(n), id_s);
-                mma_commit(s_full);
-                return true;
-            };
-            auto dp_product = [&](uint32_t n) {
-                if (!landed(v_full(n), n)) return false;
-                scores_mma<P, SUB_BYTES>(tmem + C_DP, tmem + C_DO, v_slot(n), id_s);
-                mma_commit(v_empty(n));
-                mma_commit(dp_full);
-                return true;
-            };
-            int t = walk.first();
-            bool ok = t >= 0 && bar_wait(own_ready, 0, stop, f.status, GAVE_UP_Q);
-            fence_after();
-            ok = ok && s_product(0) && dp_product(0);
-            for (uint32_t n = 0; ok; n++) {
-                const int next = walk.from(t + 1);
-                if (next >= 0) {
-                    if (!bar_wait(s_taken, n & 1, stop, f.status, GAVE_UP_S)) break;
-                    fence_after();
-                    if (!s_product(n + 1)) break;
-                }
-                // (for the first tile the wait for an emptied accumulator is over at once: the phase before the first)
-                if (!bar_wait(ds_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait(acc_taken, (n & 1) ^ 1, stop, f.status, GAVE_UP_O_EMPTY)) break;
+    } else if (warp == MMA_WARP) {
+        constexpr uint32_t id_s = idesc(GT, false), id_acc = idesc(DP, true);
+        const uint32_t e = elect(), tm = uniform(tmem), from = uniform(base);
+        auto landed = [&](uint32_t bar, uint32_t n) { return bar_wait_warp(bar, (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
+        auto keys = [&](uint32_t n) { return from + (n % SLOTS) * SLOT; };
+        auto values = [&](uint32_t n) { return from + (SLOTS + n % SLOTS) * SLOT; };
+        auto s_product = [&](uint32_t n) {
+            if (!landed(k_full(n), n)) return false;
+            scores_mma<P, SUB_BYTES>(e, tm + C_S, tm + C_Q, keys(n), id_s);
+            mma_commit(e, s_full);
+            return true;
+        };
+        auto dp_product = [&](uint32_t n) {
+            if (!landed(v_full(n), n)) return false;
+            scores_mma<P, SUB_BYTES>(e, tm + C_DP, tm + C_DO, values(n), id_s);
+            mma_commit(e, v_empty(n));
+            mma_commit(e, dp_full);
+            return true;
+        };
+        int t = uniform(walk.first());
+        bool ok = t >= 0 && bar_wait_warp(own_ready, 0, stop, f.status, GAVE_UP_Q);
+        fence_after();
+        ok = ok && s_product(0) && dp_product(0);
+        for (uint32_t n = 0; ok; n++) {
+            const int next = uniform(walk.from(t + 1));
+            if (next >= 0) {
+                if (!bar_wait_warp(s_taken, n & 1, stop, f.status, GAVE_UP_S)) break;
                 fence_after();
-                rows_mma<P, SUB_BYTES, 4>(tmem + C_DQ, tmem + C_DP, k_slot(n), id_acc);
-                mma_commit(k_empty(n));
-                mma_commit(acc_full);
-                if (next < 0 || !dp_product(n + 1)) break;
-                t = next;
+                if (!s_product(n + 1)) break;
             }
+            // (for the first tile the wait for an emptied accumulator is over at once: the phase before the first)
+            if (!bar_wait_warp(ds_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait_warp(acc_taken, (n & 1) ^ 1, stop, f.status, GAVE_UP_O_EMPTY)) break;
+            fence_after();
+            rows_mma<P, SUB_BYTES, 4>(e, tm + C_DQ, tm + C_DP, keys(n), id_acc);
+            mma_commit(e, k_empty(n));
+            mma_commit(e, acc_full);
+            if (next < 0 || !dp_product(n + 1)) break;
+            t = next;
         }
     } else {
-        const int quad = warp & 3, half = warp >> 2, row = 32 * quad + lane, q = q0 + row, pos = q + sight.shift;
+        const int quad = warp & 3, part = warp >> 2, row = 32 * quad + lane, q = q0 + row, pos = q + sight.shift;
         const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
         const bool on = q < tq && sight.query_used(pos);
         const float doc = on && sight.docs ? sight.docs[pos] : 0.f;
@@ -713,21 +720,21 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
 #pragma unroll
         for (int which = 0; which < 2; which++) {
             const Strided4& src = which ? a.dout : a.q;
-            float x[HALF];
-            load_half_row<HALF>(src.p + b * src.bs + int64_t(on ? q : 0) * src.ts + h * src.hs, half * HALF, dim, on, which ? f.dout.vec : f.q.vec, x);
-            exchange[half * ROWS + row] = largest(x);
-            pair_sync(quad);
-            own_scale[which] = tile_scale(fmaxf(exchange[row], exchange[ROWS + row]));
+            float x[SHARE];
+            load_row_part<SHARE>(src.p + b * src.bs + int64_t(on ? q : 0) * src.ts + h * src.hs, part * SHARE, dim, on, which ? f.dout.vec : f.q.vec, x);
+            exchange[part * ROWS + row] = largest(x);
+            row_sync(quad);
+            own_scale[which] = tile_scale(row_max(exchange, row));
             const float inv = 1.f / own_scale[which];
             const uint32_t column = which ? C_DO : C_Q;
-            store_halves<HALF>(lanes + column + half * HALF, x, inv);
-            pair_sync(quad);
+            store_halves<SHARE>(lanes + column + part * SHARE, x, inv);
+            row_sync(quad);
             if (which) {
 #pragma unroll
-                for (int c = 0; c < HALF; c++) length = fmaf(x[c] * inv, x[c] * inv, length);
-                exchange[half * ROWS + row] = length;
-                pair_sync(quad);
-                length = sqrtf(exchange[row] + exchange[ROWS + row]) * own_scale[1];
+                for (int c = 0; c < SHARE; c++) length = fmaf(x[c] * inv, x[c] * inv, length);
+                exchange[part * ROWS + row] = length;
+                row_sync(quad);
+                length = sqrtf(row_sum(exchange, row)) * own_scale[1];
             }
         }
         tmem_wait_store();
@@ -738,43 +745,40 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         const float most_k = __int_as_float(cells[2]), most_v = __int_as_float(cells[3]);
         const float unit = tile_scale(fabsf(a.scale) * fmaf(length, most_v, fabsf(delta)));   // of ds
         const float ds_factor = a.scale / unit, out_factor = unit * most_k;
-        float acc[HALF];
+        float acc[SHARE];
 #pragma unroll
-        for (int c = 0; c < HALF; c++) acc[c] = 0.f;
+        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
         bool ok = true;
         uint32_t n = 0;
         auto drain = [&](uint32_t tile) {
             if (!bar_wait_warp(acc_full, tile & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
             fence_after();
-#pragma unroll
-            for (int c = 0; c < HALF; c += 32) {
-                uint32_t r[32];
-                tmem_load32(lanes + C_DQ + half * HALF + c, r);
-                tmem_wait_load();
-#pragma unroll
-                for (int k = 0; k < 32; k++) acc[c + k] += __uint_as_float(r[k]);
-            }
+            uint32_t r[SHARE];
+            tmem_load(lanes + C_DQ + part * SHARE, r);
+            tmem_wait_load();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(acc_taken);
+#pragma unroll
+            for (int c = 0; c < SHARE; c++) acc[c] += __uint_as_float(r[c]);
             return true;
         };
         const int pos_first = q0 + sight.shift;
         for (int t = walk.first(); t >= 0; t = walk.from(t + 1), n++) {
-            const int k0 = t * GT + 32 * half;
+            const int k0 = t * GT + KEYS * part;
             const float k_scale = __ldg(f.k.scale + image0 + (t >> 1)), v_scale = __ldg(f.v.scale + image0 + (t >> 1));
             const float mul = own_scale[0] * k_scale * score.mul, dp_mul = own_scale[1] * v_scale, ds_mul = ds_factor * (k_scale / most_k);
-            float p[32], bend[CAP ? 32 : 1];
-            uint32_t r[32];
+            float p[KEYS], bend[CAP ? KEYS : 1];
+            uint32_t r[KEYS];
             if (!bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
-            tmem_load32(lanes + C_S + 32 * half, r);
+            tmem_load(lanes + C_S + KEYS * part, r);
             tmem_wait_load();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(s_taken);
 #pragma unroll
-            for (int c = 0; c < 32; c++) {
+            for (int c = 0; c < KEYS; c++) {
                 float s = __uint_as_float(r[c]) * mul;
                 if constexpr (CAP) {
                     const float w = tanh_exact(s);
@@ -784,28 +788,25 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                 if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(pos - k0 - c)), s);
                 p[c] = ex2(s - lse);
             }
-            if (k0 + 31 >= sight.n || sight.docs || (sight.causal && k0 + 31 > pos_first && k0 + 31 >= sight.prefix)) {
+            const int k_last = k0 + KEYS - 1;
+            if (k_last >= sight.n || sight.docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
                 const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
 #pragma unroll
-                for (int c = 0; c < 32; c++)
+                for (int c = 0; c < KEYS; c++)
                     if (c >= ahead || (sight.docs && __ldg(sight.docs + k0 + c) != doc)) p[c] = 0.f;
             }
             if (n > 0) ok = drain(n - 1);     // beside the product dP
             if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
+            tmem_load(lanes + C_DP + KEYS * part, r);
+            tmem_wait_load();
 #pragma unroll
-            for (int k = 0; k < 32; k += 16) {
-                uint32_t d[16];
-                tmem_load16(lanes + C_DP + 32 * half + k, d);
-                tmem_wait_load();
-#pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    float w = fmaf(__uint_as_float(d[c]), dp_mul, -delta) * ds_mul;
-                    if constexpr (CAP) w *= bend[k + c];
-                    p[k + c] = p[k + c] == 0.f ? 0.f : p[k + c] * w;
-                }
-                tmem_store_halves(lanes + C_DP + 32 * half + k, p + k, 1.f);
+            for (int c = 0; c < KEYS; c++) {
+                float w = fmaf(__uint_as_float(r[c]), dp_mul, -delta) * ds_mul;
+                if constexpr (CAP) w *= bend[c];
+                p[c] = p[c] == 0.f ? 0.f : p[c] * w;
             }
+            store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f);
             tmem_wait_store();
             fence_before();
             __syncwarp();
@@ -815,14 +816,14 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         if (ok && q < tq) {
             if (!on)
 #pragma unroll
-                for (int c = 0; c < HALF; c++) acc[c] = 0.f;
-            store_row_part<HALF>(a.dq + ((int64_t(b) * tq + q) * heads + h) * dim, half * HALF, dim, f.out_vec, acc, on ? out_factor : 0.f);
+                for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+            store_row_part<SHARE>(a.dq + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.out_vec, acc, on ? out_factor : 0.f);
         }
     }
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 
 // dk and dv of 128 keys, over the queries of every head that shares them.  Everything is transposed: a thread's row is a key,
@@ -863,7 +864,7 @@ struct HeadWalk {
 };
 
 // The eight warps hold 128 accumulators a thread; the registers for that come from a warpgroup that hardly needs any.
-constexpr int KEY_THREADS = 32 * 12, KEY_REGS = 168, KEY_REGS_MANY = 224, KEY_REGS_FEW = 56;
+constexpr int KEY_WARPS = 8, KEY_THREADS = 32 * (KEY_WARPS + 4), KEY_REGS = 168, KEY_REGS_MANY = 224, KEY_REGS_FEW = 56;
 static_assert(256 * KEY_REGS_MANY + 128 * KEY_REGS_FEW <= KEY_THREADS * KEY_REGS, "the split must fit what the block was launched with");
 
 template <int P, bool CAP, bool BIAS>
@@ -903,16 +904,16 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; s++) { bar_init(q_full(s), 1); bar_init(q_empty(s), 1); bar_init(o_full(s), 1); bar_init(o_empty(s), 1); }
-        bar_init(own_ready, SOFTMAX_WARPS);
+        bar_init(own_ready, KEY_WARPS);
         bar_init(own_landed, 1);
         bar_init(s_full, 1);
-        bar_init(p_ready, SOFTMAX_WARPS);
+        bar_init(p_ready, KEY_WARPS);
         bar_init(dp_full, 1);
-        bar_init(ds_ready, SOFTMAX_WARPS);
+        bar_init(ds_ready, KEY_WARPS);
         bar_init(dv_full, 1);
-        bar_init(dv_taken, SOFTMAX_WARPS);
+        bar_init(dv_taken, KEY_WARPS);
         bar_init(dk_full, 1);
-        bar_init(dk_taken, SOFTMAX_WARPS);
+        bar_init(dk_taken, KEY_WARPS);
         *stop = 0;
         cells[0] = cells[1] = cells[2] = cells[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -972,42 +973,43 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                 }
             }
         } else if (warp == 8) {
-            if (lane == 0 && any) {
-                constexpr uint32_t id_s = idesc(GT, false), id_acc = idesc(DP, true);
-                auto landed = [&](uint32_t bar, uint32_t n) { return bar_wait(bar, (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
-                auto s_product = [&](uint32_t n) {
-                    if (!landed(q_full(n), n)) return false;
-                    scores_mma<P, SUB_BYTES>(tmem + C_S, tmem + C_K, q_slot(n), id_s);
-                    mma_commit(s_full);
-                    return true;
-                };
-                auto dp_product = [&](uint32_t n) {
-                    if (!landed(o_full(n), n)) return false;
-                    if constexpr (P == 1) scores_mma<P, SUB_BYTES>(tmem + C_DP, tmem + C_V, o_slot(n), id_s);
-                    else scores_mma_ss<P, SUB_BYTES>(tmem + C_DP, base, o_slot(n), id_s);
-                    mma_commit(dp_full);
-                    return true;
-                };
-                bool ok = bar_wait(own_ready, 0, stop, f.status, GAVE_UP_Q);
-                if constexpr (P == 2) ok = ok && bar_wait(own_landed, 0, stop, f.status, GAVE_UP_DATA);
+            constexpr uint32_t id_s = idesc(GT, false), id_acc = idesc(DP, true);
+            const uint32_t e = elect(), tm = uniform(tmem), from = uniform(base);
+            auto landed = [&](uint32_t bar, uint32_t n) { return bar_wait_warp(bar, (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
+            auto queries = [&](uint32_t n) { return from + AT_DATA + (n % SLOTS) * DATA; };
+            auto gradients = [&](uint32_t n) { return from + AT_DATA + (SLOTS + n % SLOTS) * DATA; };
+            auto s_product = [&](uint32_t n) {
+                if (!landed(q_full(n), n)) return false;
+                scores_mma<P, SUB_BYTES>(e, tm + C_S, tm + C_K, queries(n), id_s);
+                mma_commit(e, s_full);
+                return true;
+            };
+            auto dp_product = [&](uint32_t n) {
+                if (!landed(o_full(n), n)) return false;
+                if constexpr (P == 1) scores_mma<P, SUB_BYTES>(e, tm + C_DP, tm + C_V, gradients(n), id_s);
+                else scores_mma_ss<P, SUB_BYTES>(e, tm + C_DP, from, gradients(n), id_s);
+                mma_commit(e, dp_full);
+                return true;
+            };
+            bool ok = any && bar_wait_warp(own_ready, 0, stop, f.status, GAVE_UP_Q);
+            if constexpr (P == 2) ok = ok && bar_wait_warp(own_landed, 0, stop, f.status, GAVE_UP_DATA);
+            fence_after();
+            ok = ok && s_product(0) && dp_product(0);
+            for (uint32_t n = 0; ok; n++) {
+                const bool more = uniform(int(at.next()));
+                const uint32_t before = (n & 1) ^ 1;   // phase of the accumulators' emptying after the tile before
+                if (!bar_wait_warp(p_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait_warp(dv_taken, before, stop, f.status, GAVE_UP_O_EMPTY)) break;
                 fence_after();
-                ok = ok && s_product(0) && dp_product(0);
-                for (uint32_t n = 0; ok; n++) {
-                    const bool more = at.next();
-                    const uint32_t before = (n & 1) ^ 1;   // phase of the accumulators' emptying after the tile before
-                    if (!bar_wait(p_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait(dv_taken, before, stop, f.status, GAVE_UP_O_EMPTY)) break;
-                    fence_after();
-                    rows_mma<P, SUB_BYTES, 4>(tmem + C_DV, tmem + C_S, o_slot(n), id_acc);
-                    mma_commit(o_empty(n));
-                    mma_commit(dv_full);
-                    if (more && !s_product(n + 1)) break;
-                    if (!bar_wait(ds_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait(dk_taken, before, stop, f.status, GAVE_UP_O_EMPTY)) break;
-                    fence_after();
-                    rows_mma<P, SUB_BYTES, 4>(tmem + C_DK, tmem + C_DP, q_slot(n), id_acc);
-                    mma_commit(q_empty(n));
-                    mma_commit(dk_full);
-                    if (!more || !dp_product(n + 1)) break;
-                }
+                rows_mma<P, SUB_BYTES, 4>(e, tm + C_DV, tm + C_S, gradients(n), id_acc);
+                mma_commit(e, o_empty(n));
+                mma_commit(e, dv_full);
+                if (more && !s_product(n + 1)) break;
+                if (!bar_wait_warp(ds_ready, n & 1, stop, f.status, GAVE_UP_P) || !bar_wait_warp(dk_taken, before, stop, f.status, GAVE_UP_O_EMPTY)) break;
+                fence_after();
+                rows_mma<P, SUB_BYTES, 4>(e, tm + C_DK, tm + C_DP, queries(n), id_acc);
+                mma_commit(e, q_empty(n));
+                mma_commit(e, dk_full);
+                if (!more || !dp_product(n + 1)) break;
             }
         }
     } else {
@@ -1021,7 +1023,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         for (int which = 0; which < (P == 1 ? 2 : 1); which++) {   // the block's own operands, in their images' units
             const Strided4& src = which ? a.v : a.k;
             float x[HALF];
-            load_half_row<HALF>(src.p + b * src.bs + int64_t(on ? j : 0) * src.ts + g * src.hs, half * HALF, dim, on, which ? f.v.vec : f.k.vec, x);
+            load_row_part<HALF>(src.p + b * src.bs + int64_t(on ? j : 0) * src.ts + g * src.hs, half * HALF, dim, on, which ? f.v.vec : f.k.vec, x);
             const uint32_t column = which ? C_V : C_K;
             store_halves<HALF>(lanes + column + half * HALF, x, 1.f / (which ? v_scale : k_scale));
         }

@@ -73,20 +73,29 @@ __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
-// the barrier arrives once every instruction issued so far by this thread has finished
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// Products are issued by a whole warp that runs in step, one lane of which (`elected`) takes the instruction: the tensor
+// instructions want their operands in uniform registers, and a value that the compiler knows to be the same in all lanes is
+// there already.  Issued from a branch that only one lane enters, every operand of every instruction is moved over first:
+// about 150 cycles an instruction, whatever its size.
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// the barrier arrives once every instruction issued so far by this lane has finished
+__device__ __forceinline__ void mma_commit(uint32_t elected, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
 }
 
 // Shared-memory descriptor, 128-byte swizzle, strides in bytes.  Its low word (address and leading stride) may be moved by
 // a distance / 16; the high word depends on the layout alone.
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFF) >> 4) | (lbo >> 4) << 16; }
 constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29;   // groups of 8 rows 1024 bytes apart
-// keeps the compiler from holding descriptors of every step of a product in registers from one product to the next
-__device__ __forceinline__ uint32_t fresh(uint32_t x) {
-    asm volatile("" : "+r"(x));
-    return x;
-}
 // fp16 operands, fp32 accumulator, M = 128; the second operand contracted over its rows (MN-major) or its columns
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_rows, int m = 128) {
     return (1u << 4) | (b_rows ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
@@ -94,23 +103,25 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_rows, int m = 128) {
 // First operand in tensor memory (lane = row, a column holds two neighbouring fp16 values), second in shared memory.
 // An operand made of halves has 16 columns for 16 elements: 8 with the high halves, then 8 with the low ones, so that it can
 // take the place of the 16 fp32 values it was made from.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
-        "mov.b64 y, {%2, %5};\n\t"
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\t"
+        "setp.ne.b32 e, %6, 0;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH) : "memory");
+        "mov.b64 y, {%2, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH), "r"(elected) : "memory");
 }
 // both operands in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\t"
+        "setp.ne.b32 e, %6, 0;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
         "mov.b64 x, {%1, %5};\n\t"
         "mov.b64 y, {%2, %5};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH) : "memory");
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(DESC_HIGH), "r"(elected) : "memory");
 }
 
 // 32 columns of the warp's 32 lanes; the values may be used after tmem_wait_load
@@ -133,6 +144,8 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_load32(taddr, r); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) { tmem_load16(taddr, r); }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
