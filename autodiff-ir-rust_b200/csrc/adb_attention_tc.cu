@@ -163,6 +163,19 @@ struct Walk {
     __device__ __forceinline__ int first() const { return from(begin); }
 };
 
+// Blocks that own queries: heads go in rounds whose keys and values fit into L2 together; within a round the longest tiles of
+// all heads start first, so that the SMs finish together.
+__device__ __forceinline__ void own_tile(int heads, int round, int tiles, int& bh, int& tile) {
+    const int first = int(blockIdx.x / unsigned(round * tiles)) * round, in = int(blockIdx.x) - first * tiles, n = min(round, heads - first);
+    bh = first + in % n;
+    tile = tiles - 1 - in / n;
+}
+int heads_in_round(const AttentionShape& s, int P) {
+    const int64_t bytes = 2 * ((s.tk + ROWS - 1) / ROWS) * image_bytes(P), most = s.batch * s.heads;   // of one key head
+    const int64_t n = (int64_t(48) << 20) / bytes * (s.heads / s.kv_heads);
+    return int(std::max<int64_t>(1, std::min(n, most)));
+}
+
 enum : int { GAVE_UP_Q = ATTENTION_GAVE_UP, GAVE_UP_SLOT, GAVE_UP_DATA, GAVE_UP_S, GAVE_UP_P, GAVE_UP_O_FULL, GAVE_UP_O_EMPTY };
 
 // a thread's share of a row as fp32, zero outside
@@ -286,7 +299,7 @@ struct ForwardArgs {
     const float *k_scale, *v_scale;
     const float2* doc_range;
     int* status;
-    int q_vec, o_vec;
+    int q_vec, o_vec, round;
 };
 
 template <int P>
@@ -320,8 +333,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tq = int(a.s.tq), dim = int(a.s.dim), heads = int(a.s.heads), kv_heads = int(a.s.kv_heads);
     const int q_tiles = (tq + ROWS - 1) / ROWS, k_tiles = (int(a.s.tk) + KT - 1) / KT;
-    const int bh = int(blockIdx.x / q_tiles), b = bh / heads, h = bh % heads, g = h / (heads / kv_heads);
-    const int q0 = (q_tiles - 1 - int(blockIdx.x % q_tiles)) * ROWS;   // the longest tiles of a head start first
+    int bh, tile;
+    own_tile(int(a.s.batch) * heads, f.round, q_tiles, bh, tile);
+    const int b = bh / heads, h = bh % heads, g = h / (heads / kv_heads), q0 = tile * ROWS;
     const Sight sight(a, b);
 
     if (threadIdx.x == 0) {
@@ -555,7 +569,7 @@ struct GradArgs {
     AttentionArgs a;
     ImageJob k, v, q, dout;
     int* status;
-    int out_vec;
+    int out_vec, round;
 };
 
 // half an image (64 rows): a piece for each half and panel
@@ -611,8 +625,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tq = int(a.s.tq), dim = int(a.s.dim), heads = int(a.s.heads), kv_heads = int(a.s.kv_heads);
     const int q_tiles = f.q.tiles, k_tiles = f.k.tiles;
-    const int bh = int(blockIdx.x / q_tiles), b = bh / heads, h = bh % heads, g = h / (heads / kv_heads);
-    const int q0 = (q_tiles - 1 - int(blockIdx.x % q_tiles)) * ROWS;
+    int bh, tile;
+    own_tile(int(a.s.batch) * heads, f.round, q_tiles, bh, tile);
+    const int b = bh / heads, h = bh % heads, g = h / (heads / kv_heads), q0 = tile * ROWS;
     const Sight sight(a, b);
     const int64_t image0 = (int64_t(b) * kv_heads + g) * k_tiles;
     const int keys_end = max(sight.keys_end(min(q0 + ROWS, tq) - 1 + sight.shift), 0);
@@ -863,14 +878,15 @@ struct HeadWalk {
     }
 };
 
-// The eight warps hold 128 accumulators a thread; the registers for that come from a warpgroup that hardly needs any.
-constexpr int KEY_WARPS = 8, KEY_THREADS = 32 * (KEY_WARPS + 4), KEY_REGS = 168, KEY_REGS_MANY = 224, KEY_REGS_FEW = 56;
-static_assert(256 * KEY_REGS_MANY + 128 * KEY_REGS_FEW <= KEY_THREADS * KEY_REGS, "the split must fit what the block was launched with");
+// The arithmetic's warps hold 64 accumulators a thread; some of the registers for that come from a warpgroup that hardly
+// needs any.
+constexpr int KEY_THREADS = 32 * (SOFTMAX_WARPS + 4), KEY_REGS = 96, KEY_REGS_MANY = 112, KEY_REGS_FEW = 32;
+static_assert(32 * SOFTMAX_WARPS * KEY_REGS_MANY + 128 * KEY_REGS_FEW <= KEY_THREADS * KEY_REGS, "the split must fit what the block was launched with");
 
 template <int P, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const GradArgs f) {
     using Shared = KeyGradShared<P>;
-    constexpr int SLOTS = Shared::SLOTS, DATA = Shared::DATA_BYTES, STATS = Shared::STATS_BYTES, DP = 64 * P, HALF = DP / 2;
+    constexpr int SLOTS = Shared::SLOTS, DATA = Shared::DATA_BYTES, STATS = Shared::STATS_BYTES, DP = 64 * P, SHARE = DP / PARTS, QUERIES = GT / PARTS;
     constexpr uint32_t C_K = 0, C_DK = DP, C_DV = 2 * DP, C_S = 3 * DP, C_DP = 3 * DP + 64, C_V = 3 * DP + 128;   // C_V: one panel only
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -904,21 +920,21 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; s++) { bar_init(q_full(s), 1); bar_init(q_empty(s), 1); bar_init(o_full(s), 1); bar_init(o_empty(s), 1); }
-        bar_init(own_ready, KEY_WARPS);
+        bar_init(own_ready, SOFTMAX_WARPS);
         bar_init(own_landed, 1);
         bar_init(s_full, 1);
-        bar_init(p_ready, KEY_WARPS);
+        bar_init(p_ready, SOFTMAX_WARPS);
         bar_init(dp_full, 1);
-        bar_init(ds_ready, KEY_WARPS);
+        bar_init(ds_ready, SOFTMAX_WARPS);
         bar_init(dv_full, 1);
-        bar_init(dv_taken, KEY_WARPS);
+        bar_init(dv_taken, SOFTMAX_WARPS);
         bar_init(dk_full, 1);
-        bar_init(dk_taken, KEY_WARPS);
+        bar_init(dk_taken, SOFTMAX_WARPS);
         *stop = 0;
         cells[0] = cells[1] = cells[2] = cells[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
+    if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
     __syncthreads();
     block_max(&cells[0], f.q.scale + head0 * q_tiles, group * q_tiles);
     block_max(&cells[1], f.dout.scale + head0 * q_tiles, group * q_tiles);
@@ -941,9 +957,9 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     HeadWalk at;
     const bool any = at.start(walk, 0, group);
 
-    if (warp >= 8) {
+    if (warp >= MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KEY_REGS_FEW));
-        if (warp == 9) {
+        if (warp == LOAD_WARP) {
             if (lane == 0 && any) {
                 if constexpr (P == 2) {
                     bar_expect(own_landed, image_bytes(P));
@@ -972,7 +988,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                         for (uint32_t it = 0; it < SPIN_LIMIT && !bar_test(own_landed, 0); it++) __nanosleep(64);
                 }
             }
-        } else if (warp == 8) {
+        } else if (warp == MMA_WARP) {
             constexpr uint32_t id_s = idesc(GT, false), id_acc = idesc(DP, true);
             const uint32_t e = elect(), tm = uniform(tmem), from = uniform(base);
             auto landed = [&](uint32_t bar, uint32_t n) { return bar_wait_warp(bar, (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA); };
@@ -1014,7 +1030,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KEY_REGS_MANY));
-        const int quad = warp & 3, half = warp >> 2, row = 32 * quad + lane, j = k0 + row;
+        const int quad = warp & 3, part = warp >> 2, row = 32 * quad + lane, j = k0 + row;
         const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
         const bool on = j < tk && sight.key_used(j);
         const float doc = on && sight.docs ? sight.docs[j] : 0.f;
@@ -1022,10 +1038,10 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
 #pragma unroll
         for (int which = 0; which < (P == 1 ? 2 : 1); which++) {   // the block's own operands, in their images' units
             const Strided4& src = which ? a.v : a.k;
-            float x[HALF];
-            load_row_part<HALF>(src.p + b * src.bs + int64_t(on ? j : 0) * src.ts + g * src.hs, half * HALF, dim, on, which ? f.v.vec : f.k.vec, x);
+            float x[SHARE];
+            load_row_part<SHARE>(src.p + b * src.bs + int64_t(on ? j : 0) * src.ts + g * src.hs, part * SHARE, dim, on, which ? f.v.vec : f.k.vec, x);
             const uint32_t column = which ? C_V : C_K;
-            store_halves<HALF>(lanes + column + half * HALF, x, 1.f / (which ? v_scale : k_scale));
+            store_halves<SHARE>(lanes + column + part * SHARE, x, 1.f / (which ? v_scale : k_scale));
         }
         tmem_wait_store();
         fence_before();
@@ -1038,19 +1054,19 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         const int64_t out_row = ((int64_t(b) * tk + j) * kv_heads + g) * dim;
         bool ok = true;
         uint32_t n = 0;
-        float dk[HALF], dv[HALF];
+        float dk[SHARE], dv[SHARE];
 #pragma unroll
-        for (int c = 0; c < HALF; c++) dk[c] = dv[c] = 0.f;
-        auto drain = [&](uint32_t full, uint32_t taken, uint32_t column, uint32_t tile, float (&acc)[HALF]) {
+        for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
+        auto drain = [&](uint32_t full, uint32_t taken, uint32_t column, uint32_t tile, float (&acc)[SHARE]) {
             if (!bar_wait_warp(full, tile & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
             fence_after();
 #pragma unroll
-            for (int c = 0; c < HALF; c += 32) {
-                uint32_t r[32];
-                tmem_load32(lanes + column + half * HALF + c, r);
+            for (int c = 0; c < SHARE; c += 16) {   // (16 at a time: registers)
+                uint32_t r[16];
+                tmem_load(lanes + column + part * SHARE + c, r);
                 tmem_wait_load();
 #pragma unroll
-                for (int k = 0; k < 32; k++) acc[c + k] += __uint_as_float(r[k]);
+                for (int k = 0; k < 16; k++) acc[c + k] += __uint_as_float(r[k]);
             }
             fence_before();
             __syncwarp();
@@ -1058,27 +1074,27 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             return true;
         };
         for (bool more = any; more; more = at.next(), n++) {
-            const int q0 = at.t * GT + 32 * half;   // the thread's first query
+            const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
             const int64_t image = (head0 + at.head) * q_tiles + (at.t >> 1);
             const ScoreOf score(a, g * group + at.head);
             const float q_scale = __ldg(f.q.scale + image), o_scale = __ldg(f.dout.scale + image);
             const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale, ds_mul = ds_factor * (q_scale / most_q), p_mul = 1024.f * (o_scale / most_o);
             if (!ok || !bar_wait_warp(q_full(n), (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA) || !bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
-            const float4* lse = reinterpret_cast<const float4*>(gen + stats(n)) + 8 * half;
+            const float4* lse = reinterpret_cast<const float4*>(gen + stats(n)) + QUERIES / 4 * part;
             const float4* delta = lse + GT / 4;
             const bool partly = sight.docs || (sight.causal && q0 + sight.shift < k0 + ROWS - 1 && k0 + ROWS - 1 >= sight.prefix);
             const int behind = sight.causal && j >= sight.prefix ? j - sight.shift - q0 : 0;   // queries in front of the key
-            float p[32];      // weights, times the scores' bend once they are stored
-#pragma unroll
-            for (int k = 0; k < 32; k += 16) {
-                uint32_t r[16];
-                float x[16];
-                tmem_load16(lanes + C_S + 32 * half + k, r);
+            static_assert(QUERIES == 16, "a thread's columns of a tile");
+            float p[QUERIES];      // weights, times the scores' bend once they are stored
+            uint32_t r[QUERIES];
+            {
+                float x[QUERIES];
+                tmem_load(lanes + C_S + QUERIES * part, r);
                 tmem_wait_load();
 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    const float4 ls = lse[(k + c) / 4];
+                for (int c = 0; c < QUERIES; c += 4) {
+                    const float4 ls = lse[c / 4];
                     const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -1088,17 +1104,17 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                             bend = fmaf(-w, w, 1.f);
                             s = score.cap2 * w;
                         }
-                        if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(q0 + k + c + e + sight.shift - j)), s);
+                        if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(q0 + c + e + sight.shift - j)), s);
                         float w = ex2(s - l4[e]);
                         if (partly) {
-                            const int q = q0 + k + c + e;
-                            if (k + c + e < behind || (sight.docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
+                            const int q = q0 + c + e;
+                            if (c + e < behind || (sight.docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
                         }
                         x[c + e] = w * p_mul;
-                        p[k + c + e] = CAP ? w * bend : w;
+                        p[c + e] = CAP ? w * bend : w;
                     }
                 }
-                tmem_store_halves(lanes + C_S + 32 * half + k, x, 1.f);
+                store_halves<QUERIES>(lanes + C_S + QUERIES * part, x, 1.f);
             }
             tmem_wait_store();
             fence_before();
@@ -1107,23 +1123,19 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             if (n > 0) ok = drain(dk_full, dk_taken, C_DK, n - 1, dk);   // beside the product dP
             if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
+            tmem_load(lanes + C_DP + QUERIES * part, r);
+            tmem_wait_load();
 #pragma unroll
-            for (int k = 0; k < 32; k += 16) {
-                uint32_t r[16];
-                tmem_load16(lanes + C_DP + 32 * half + k, r);
-                tmem_wait_load();
+            for (int c = 0; c < QUERIES; c += 4) {
+                const float4 de = delta[c / 4];
+                const float d4[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    const float4 de = delta[(k + c) / 4];
-                    const float d4[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float w = fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]) * ds_mul;
-                        p[k + c + e] = p[k + c + e] == 0.f ? 0.f : p[k + c + e] * w;
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const float w = fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]) * ds_mul;
+                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * w;
                 }
-                tmem_store_halves(lanes + C_DP + 32 * half + k, p + k, 1.f);
             }
+            store_halves<QUERIES>(lanes + C_DP + QUERIES * part, p, 1.f);
             tmem_wait_store();
             fence_before();
             __syncwarp();
@@ -1134,15 +1146,15 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         if (ok && j < tk) {
             if (!on)   // no query sees the key, whatever its row was compared with
 #pragma unroll
-                for (int c = 0; c < HALF; c++) dk[c] = dv[c] = 0.f;
-            if (a.dk) store_row_part<HALF>(a.dk + out_row, half * HALF, dim, f.out_vec, dk, on ? dk_factor : 0.f);
-            if (a.dv) store_row_part<HALF>(a.dv + out_row, half * HALF, dim, f.out_vec, dv, on ? dv_factor : 0.f);
+                for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
+            if (a.dk) store_row_part<SHARE>(a.dk + out_row, part * SHARE, dim, f.out_vec, dk, on ? dk_factor : 0.f);
+            if (a.dv) store_row_part<SHARE>(a.dv + out_row, part * SHARE, dim, f.out_vec, dv, on ? dv_factor : 0.f);
         }
     }
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 
 bool fits16(const Strided4& t, int64_t dim) {
@@ -1239,6 +1251,7 @@ int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string
         f.status = a.status;
         f.q_vec = fits16(a.q, s.dim);
         f.o_vec = aligned_rows(a.o, s.dim);
+        f.round = heads_in_round(s, P);
         const unsigned blocks = unsigned(s.batch * s.heads * ((s.tq + ROWS - 1) / ROWS));
         e = P == 1 ? forward<1>(f, blocks, stream) : forward<2>(f, blocks, stream);
     }
@@ -1271,6 +1284,7 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
     f.a = a;
     f.k = im.job[0]; f.v = im.job[1]; f.q = im.job[2]; f.dout = im.job[3];
     f.status = a.status;
+    f.round = heads_in_round(s, P);
     if (e == cudaSuccess && a.dq) {
         f.out_vec = aligned_rows(a.dq, s.dim);
         const unsigned blocks = unsigned(s.batch * s.heads * q_tiles);
