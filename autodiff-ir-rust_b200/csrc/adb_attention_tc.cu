@@ -464,9 +464,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         };
         int i = 0;
         const int pos_first = q0 + sight.shift;
-        for (int t = walk.first(); t >= 0; t = walk.from(t + 1), i++) {
+        int t = walk.first();
+        float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
+        for (int next; t >= 0; t = next, i++) {
             const int k0 = t * KT + KEYS * part;
-            const float mul = q_scale * __ldg(f.k_scale + image0 + t) * score.mul, v_scale = __ldg(f.v_scale + image0 + t);
+            const float mul = q_scale * k_next * score.mul, v_scale = v_next;
+            next = walk.from(t + 1);
+            if (next >= 0) {   // a tile ahead: a load takes longer than the waits below should
+                k_next = __ldg(f.k_scale + image0 + next);
+                v_next = __ldg(f.v_scale + image0 + next);
+            }
             // a warp that gives up still meets the others once, so that none waits for it for good
             ok = ok && bar_wait_warp(s_full(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_S);
             fence_after();
@@ -779,9 +786,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             return true;
         };
         const int pos_first = q0 + sight.shift;
-        for (int t = walk.first(); t >= 0; t = walk.from(t + 1), n++) {
+        int t = walk.first();
+        float k_next = t >= 0 ? __ldg(f.k.scale + image0 + (t >> 1)) : 0.f, v_next = t >= 0 ? __ldg(f.v.scale + image0 + (t >> 1)) : 0.f;
+        for (int next; t >= 0; t = next, n++) {
             const int k0 = t * GT + KEYS * part;
-            const float k_scale = __ldg(f.k.scale + image0 + (t >> 1)), v_scale = __ldg(f.v.scale + image0 + (t >> 1));
+            const float k_scale = k_next, v_scale = v_next;
+            next = walk.from(t + 1);
+            if (next >= 0) {   // a tile ahead
+                k_next = __ldg(f.k.scale + image0 + (next >> 1));
+                v_next = __ldg(f.v.scale + image0 + (next >> 1));
+            }
             const float mul = own_scale[0] * k_scale * score.mul, dp_mul = own_scale[1] * v_scale, ds_mul = ds_factor * (k_scale / most_k);
             float p[KEYS], bend[CAP ? KEYS : 1];
             uint32_t r[KEYS];
@@ -1073,11 +1087,20 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             if (lane == 0) bar_arrive(taken);
             return true;
         };
-        for (bool more = any; more; more = at.next(), n++) {
-            const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
+        float q_next = 0.f, o_next = 0.f, slope_next = 0.f;
+        auto look = [&]() {   // what belongs to the tile of queries that `at` stands on
             const int64_t image = (head0 + at.head) * q_tiles + (at.t >> 1);
-            const ScoreOf score(a, g * group + at.head);
-            const float q_scale = __ldg(f.q.scale + image), o_scale = __ldg(f.dout.scale + image);
+            q_next = __ldg(f.q.scale + image);
+            o_next = __ldg(f.dout.scale + image);
+            if constexpr (BIAS) slope_next = __ldg(a.slopes + g * group + at.head) * LOG2E;
+        };
+        if (any) look();
+        const ScoreOf score(a, g * group);   // (but for the slope the same for every head)
+        for (bool more = any; more; n++) {
+            const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
+            const float q_scale = q_next, o_scale = o_next, slope2 = slope_next;
+            more = at.next();
+            if (more) look();   // a tile ahead
             const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale, ds_mul = ds_factor * (q_scale / most_q), p_mul = 1024.f * (o_scale / most_o);
             if (!ok || !bar_wait_warp(q_full(n), (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA) || !bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
@@ -1104,7 +1127,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                             bend = fmaf(-w, w, 1.f);
                             s = score.cap2 * w;
                         }
-                        if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(q0 + c + e + sight.shift - j)), s);
+                        if constexpr (BIAS) s = fmaf(-slope2, fabsf(float(q0 + c + e + sight.shift - j)), s);
                         float w = ex2(s - l4[e]);
                         if (partly) {
                             const int q = q0 + c + e;
