@@ -46,10 +46,12 @@ struct ImageArgs {
     ImageJob job[4];
 };
 
+constexpr int IMAGE_WARPS = 16;
+
 template <int P>
-__global__ void __launch_bounds__(256) adb_attention_images(const ImageArgs args) {
-    constexpr int LPR = 16 * P, RPW = 32 / LPR, N = ROWS / 8 / RPW;   // lanes of a row, rows a warp reads at a time, times
-    __shared__ float most[8], longest[8];
+__global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(const ImageArgs args) {
+    constexpr int LPR = 16 * P, RPW = 32 / LPR, RUN = ROWS / IMAGE_WARPS, N = RUN / RPW;   // lanes of a row, rows a warp reads at a time, rows of a warp, times
+    __shared__ float most[IMAGE_WARPS], longest[IMAGE_WARPS];
     __shared__ int doc_lo, doc_hi;
     const ImageJob& job = args.job[blockIdx.z];
     const int tile = blockIdx.x, bh = blockIdx.y;
@@ -72,40 +74,45 @@ __global__ void __launch_bounds__(256) adb_attention_images(const ImageArgs args
         }
         return x;
     };
+    auto token = [&](int i) { return tile * ROWS + warp * RUN + i * RPW + lane / LPR; };
+    auto used = [&](int t) { return t < job.tokens && (job.of_keys ? sight.key_used(t) : sight.query_used(t + sight.shift)); };
+    const int64_t padded0 = int64_t(bh) * job.tiles * ROWS;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int t = tile * ROWS + warp * (ROWS / 8) + i * RPW + lane / LPR;
-        const bool used = t < job.tokens && (job.of_keys ? sight.key_used(t) : sight.query_used(t + sight.shift));
-        v[i] = used ? quad(src + int64_t(t) * job.src.ts + c, job.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const int64_t padded_row = int64_t(bh) * job.tiles * ROWS + t;
-        if (job.lse && lane % LPR == 0) {
-            const float x = used ? __ldg(args.a.lse_in + int64_t(bh) * job.tokens + t) : -INFINITY;
-            job.lse[padded_row] = x == -INFINITY ? INFINITY : x;
-        }
-        if (job.delta) {
-            float s = 0.f;
-            if (used) {
-                const float4 o = quad(args.a.out.p + b * args.a.out.bs + int64_t(t) * args.a.out.ts + h * args.a.out.hs + c, args.a.out_vec);
-                s = fmaf(v[i].x, o.x, fmaf(v[i].y, o.y, fmaf(v[i].z, o.z, v[i].w * o.w)));
-            }
+    for (int i = 0; i < N; i++) v[i] = used(token(i)) ? quad(src + int64_t(token(i)) * job.src.ts + c, job.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (job.delta) {
+        const float* out = args.a.out.p + b * args.a.out.bs + h * args.a.out.hs + c;
+        float4 o[N];
 #pragma unroll
-            for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (lane % LPR == 0) job.delta[padded_row] = s;
+        for (int i = 0; i < N; i++) o[i] = used(token(i)) ? quad(out + int64_t(token(i)) * args.a.out.ts, args.a.out_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float s = fmaf(v[i].x, o[i].x, fmaf(v[i].y, o[i].y, fmaf(v[i].z, o[i].z, v[i].w * o[i].w)));
+#pragma unroll
+            for (int m = LPR / 2; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+            if (lane % LPR == 0) job.delta[padded0 + token(i)] = s;
         }
-        top = fmaxf(fmaxf(fmaxf(top, finite_magnitude(v[i].x)), finite_magnitude(v[i].y)), fmaxf(finite_magnitude(v[i].z), finite_magnitude(v[i].w)));
     }
+    if (job.lse)
+        for (int r = threadIdx.x; r < ROWS; r += 32 * IMAGE_WARPS) {
+            const int t = tile * ROWS + r;
+            const float x = used(t) ? __ldg(args.a.lse_in + int64_t(bh) * job.tokens + t) : -INFINITY;
+            job.lse[padded0 + t] = x == -INFINITY ? INFINITY : x;
+        }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        top = fmaxf(fmaxf(fmaxf(top, finite_magnitude(v[i].x)), finite_magnitude(v[i].y)), fmaxf(finite_magnitude(v[i].z), finite_magnitude(v[i].w)));
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) most[warp] = top;
     if (threadIdx.x == 0) { doc_lo = 0x7fffffff; doc_hi = -1; }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; w++) top = fmaxf(top, most[w]);
+    for (int w = 0; w < IMAGE_WARPS; w++) top = fmaxf(top, most[w]);
     const float scale = tile_scale(top), inv = 1.f / scale;
     uint8_t* image = job.image + (int64_t(bh) * job.tiles + tile) * image_bytes(P);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int row = warp * (ROWS / 8) + i * RPW + lane / LPR;
+        const int row = warp * RUN + i * RPW + lane / LPR;
         uint2 hi, lo;
         const float4 x = make_float4(v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv);
         halves(x.x, x.y, hi.x, lo.x);
@@ -140,7 +147,7 @@ __global__ void __launch_bounds__(256) adb_attention_images(const ImageArgs args
     if (job.norm) {
         float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; w++) l = fmaxf(l, longest[w]);
+        for (int w = 0; w < IMAGE_WARPS; w++) l = fmaxf(l, longest[w]);
         job.norm[int64_t(bh) * job.tiles + tile] = sqrtf(l) * scale;
     }
     if (ranges) job.docs[int64_t(b) * job.tiles + tile] = doc_hi < 0 ? make_float2(INFINITY, -1.f) : make_float2(__int_as_float(doc_lo), __int_as_float(doc_hi));
@@ -1230,8 +1237,8 @@ cudaError_t images(const ImageArgs& im, int jobs, int P, CUstream_st* stream) {
         x = std::max(x, unsigned(im.job[i].tiles));
         y = std::max(y, unsigned(im.a.s.batch * im.job[i].heads));
     }
-    if (P == 1) adb_attention_images<1><<<dim3(x, y, unsigned(jobs)), 256, 0, stream>>>(im);
-    else adb_attention_images<2><<<dim3(x, y, unsigned(jobs)), 256, 0, stream>>>(im);
+    if (P == 1) adb_attention_images<1><<<dim3(x, y, unsigned(jobs)), 32 * IMAGE_WARPS, 0, stream>>>(im);
+    else adb_attention_images<2><<<dim3(x, y, unsigned(jobs)), 32 * IMAGE_WARPS, 0, stream>>>(im);
     return cudaGetLastError();
 }
 template <int P, bool KEYS>
