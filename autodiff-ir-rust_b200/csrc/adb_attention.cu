@@ -356,7 +356,7 @@ int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& e
 }
 
 int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err) {
-    if (attention_uses_tc(a.s)) return attention_tc_grad_launch(a, stream, err);
+    if (attention_grad_uses_tc(a.s)) return attention_tc_grad_launch(a, stream, err);
     const int dim = int(a.s.dim), ld = padded(dim);
     const Vec vec{fits16(a.q, dim), fits16(a.k, dim), fits16(a.v, dim), false, fits16(a.dout, dim)};
     const int T = dim <= 128 ? 64 : 32;

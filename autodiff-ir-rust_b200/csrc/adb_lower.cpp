@@ -1575,6 +1575,7 @@ class Lowerer {
         if (Tq >= (int64_t(1) << 24) || Tk >= (int64_t(1) << 24)) fail("Attention: more than 2^24 tokens");
         // grids count tiles of 32 tokens of every head in 31 bits
         if (double(B) * double(H) * double(std::max(Tq, Tk) / 32 + 1) > 2e9) fail("Attention: more than 2^31 tiles");
+        if (B * H * Tq >= (int64_t(1) << 31)) fail("Attention: more than 2^31 rows");
         const Shape ls{B, H, Tq};
         if (grad) {
             Node *out = operand(c, 7), *lse = operand(c, 8), *dout = operand(c, 9);

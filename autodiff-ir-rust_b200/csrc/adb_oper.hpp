@@ -97,8 +97,13 @@ inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
     const int64_t tiles = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, n = s.batch * s.kv_heads * tiles;
     return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64;
 }
+// The gradient takes them whatever the count of queries (a tile of 128 is padded): for one query against 60000 keys the
+// CUDA-core kernels, with their 64-row tiles just as empty, need four times as long.
+inline bool attention_grad_uses_tc(const AttentionShape& s) {
+    return s.dim <= ATTENTION_TC_MAX_DIM && s.tk >= 64 && s.batch * s.heads <= 65535;
+}
 inline int64_t attention_grad_workspace(const AttentionShape& s) {
-    if (!attention_uses_tc(s)) return s.batch * s.heads * s.tq;   // one number per query: the gradient of the output times the output
+    if (!attention_grad_uses_tc(s)) return s.batch * s.heads * s.tq;   // one number per query: the gradient of the output times the output
     const int64_t kt = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, qt = (s.tq + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE;
     const int64_t nk = s.batch * s.kv_heads * kt, nq = s.batch * s.heads * qt;
     // images of four operands with their scales, two norms, logarithms and deltas in whole tiles, document numbers

@@ -522,7 +522,7 @@ class Executor {
             a.work = work;
             a.status = d_->gemm.status;
             a.sm_count = d_->sm_count;
-            if (attention_uses_tc(a.s)) oper_tc_++;
+            if (grad ? attention_grad_uses_tc(a.s) : attention_uses_tc(a.s)) oper_tc_++;
             if (!grad) {
                 a.o = out(0); a.lse = out(1);
                 return attention_launch(a, cur_stream_, err);

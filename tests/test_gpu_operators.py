@@ -207,6 +207,13 @@ def test_few_queries_against_a_cache(b, tq, tk, h, g, d, kw):
     oc.attention_check(oc.attention_run(b200(), c, grad=False), c)
 
 
+@pytest.mark.parametrize("tq,tk,h,g,d,kw", [(1, 64, 2, 1, 64, {}), (5, 700, 6, 2, 128, dict(cap=8.0)), (20, 300, 2, 2, 40, dict(slopes=True)),
+                                            (1, 63, 2, 2, 64, {}), (3, 200, 4, 1, 130, dict(causal=False))])
+def test_gradient_of_few_queries(tq, tk, h, g, d, kw):
+    c = oc.attention_case(2, tq, tk, h, g, d, seed=tq, **kw)
+    oc.attention_check(oc.attention_run(b200(), c), c)
+
+
 def test_a_cache_beyond_two_to_the_31_bytes():
     """offsets into keys pass 2^31 bytes: the last sequence's rows are the ones that count"""
     torch = pytest.importorskip("torch")
