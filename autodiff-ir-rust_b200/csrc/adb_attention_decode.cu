@@ -273,6 +273,10 @@ cudaError_t split(const AttentionArgs& a, int rows, int64_t blocks_of_one, int r
 
 }  // namespace
 
+void attention_join(const AttentionArgs& a, int ranges, const float* partial, CUstream_st* stream) {
+    adb_attention_join<<<unsigned(a.s.batch * a.s.tq * a.s.heads), 128, 0, stream>>>(a, ranges, partial);
+}
+
 int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err) {
     const AttentionShape& s = a.s;
     const int rows = int(s.heads / s.kv_heads * s.tq), ranges = int(attention_ranges(s, a.sm_count)), keys = int(attention_range_keys(s, a.sm_count));
@@ -283,7 +287,7 @@ int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::str
                     : s.dim <= 128 ? split<4>(a, rows, blocks, ranges, keys, stream)
                                    : split<8>(a, rows, blocks, ranges, keys, stream);
     if (e == cudaSuccess && ranges > 1) {
-        adb_attention_join<<<unsigned(s.batch * s.tq * s.heads), 128, 0, stream>>>(a, ranges, a.work);
+        attention_join(a, ranges, a.work, stream);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess) return ranges > 1 ? 2 : 1;

@@ -168,6 +168,12 @@ struct Walk {
         return -1;
     }
     __device__ __forceinline__ int first() const { return from(begin); }
+    // what block blockIdx.y of gridDim.y takes of the walk
+    __device__ __forceinline__ void share() {
+        const int n = max(end - begin, 0), at = begin;
+        begin = at + int(int64_t(n) * blockIdx.y / gridDim.y);
+        end = at + int(int64_t(n) * (blockIdx.y + 1) / gridDim.y);
+    }
 };
 
 // Blocks that own queries: heads go in rounds whose keys and values fit into L2 together; within a round the longest tiles of
@@ -307,6 +313,7 @@ struct ForwardArgs {
     const float2* doc_range;
     int* status;
     int q_vec, o_vec, round;
+    float* partial;   // of blocks that share a tile
 };
 
 template <int P>
@@ -376,6 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     walk.range = sight.docs ? f.doc_range + int64_t(b) * k_tiles : nullptr;
     walk.lo = sight.docs && doc_span[1] < 0 ? INFINITY : __int_as_float(doc_span[0]);
     walk.hi = doc_span[1] < 0 ? -1.f : __int_as_float(doc_span[1]);
+    walk.share();
     const int64_t image0 = (int64_t(b) * kv_heads + g) * k_tiles;
 
     if (warp == LOAD_WARP) {
@@ -548,13 +556,23 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             l = row_sum(cell, row);
             if (q < tq) {
                 const bool any = on && l != 0.f;
-                if (a.o) {
+                if (gridDim.y > 1) {   // a share of the keys: joined with the others later
+                    float* p = f.partial + ((((int64_t(b) * tq + q) * heads + h) * gridDim.y) + blockIdx.y) * (dim + 2);
+                    if (!any)
+#pragma unroll
+                        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+                    store_row_part<SHARE>(p, part * SHARE, dim, false, acc, 1.f);
+                    if (part == 0) {
+                        p[dim] = any ? m - P_SHIFT : -INFINITY;
+                        p[dim + 1] = any ? l : 0.f;
+                    }
+                } else if (a.o) {
                     if (!any)
 #pragma unroll
                         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
                     store_row_part<SHARE>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
                 }
-                if (a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + (log2f(l) - P_SHIFT) : -INFINITY;
+                if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + (log2f(l) - P_SHIFT) : -INFINITY;
             }
         }
     }
@@ -584,6 +602,7 @@ struct GradArgs {
     ImageJob k, v, q, dout;
     int* status;
     int out_vec, round;
+    float *dq, *dk, *dv;   // the results, or the parts of blocks that share a tile, one behind the other
 };
 
 // half an image (64 rows): a piece for each half and panel
@@ -673,6 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
     walk.begin = 0;
     walk.halves = 1;
     walk.end = (keys_end + GT - 1) / GT;
+    walk.share();
     walk.range = sight.docs ? f.k.docs + int64_t(b) * k_tiles : nullptr;
     if (sight.docs) {
         const float2 own = __ldg(f.q.docs + int64_t(b) * q_tiles + q0 / ROWS);
@@ -853,7 +873,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             if (!on)
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-            store_row_part<SHARE>(a.dq + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.out_vec, acc, on ? out_factor : 0.f);
+            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, on ? out_factor : 0.f);
         }
     }
     fence_before();
@@ -969,6 +989,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     walk.halves = 1;
     walk.begin = sight.causal && k0 >= sight.prefix ? max(0, k0 - sight.shift) / GT : 0;
     walk.end = k0 < sight.n ? (tq + GT - 1) / GT : 0;
+    walk.share();
     walk.range = sight.docs ? f.q.docs + int64_t(b) * q_tiles : nullptr;
     if (sight.docs) {
         const float2 own = __ldg(f.k.docs + int64_t(b) * k_tiles + tile);
@@ -1072,7 +1093,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         const float unit = tile_scale(fabsf(a.scale) * norm_o * (__ldg(f.v.norm + own_image) + norm_v));   // of ds
         const float ds_factor = a.scale / unit, dk_factor = unit * most_q;
         const float dv_factor = most_o * (1.f / 1024.f);
-        const int64_t out_row = ((int64_t(b) * tk + j) * kv_heads + g) * dim;
+        const int64_t out_row = (((int64_t(blockIdx.y) * a.s.batch + b) * tk + j) * kv_heads + g) * dim;
         bool ok = true;
         uint32_t n = 0;
         float dk[SHARE], dv[SHARE];
@@ -1177,8 +1198,8 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             if (!on)   // no query sees the key, whatever its row was compared with
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
-            if (a.dk) store_row_part<SHARE>(a.dk + out_row, part * SHARE, dim, f.out_vec, dk, on ? dk_factor : 0.f);
-            if (a.dv) store_row_part<SHARE>(a.dv + out_row, part * SHARE, dim, f.out_vec, dv, on ? dv_factor : 0.f);
+            if (f.dk) store_row_part<SHARE>(f.dk + out_row, part * SHARE, dim, f.out_vec, dk, on ? dk_factor : 0.f);
+            if (f.dv) store_row_part<SHARE>(f.dv + out_row, part * SHARE, dim, f.out_vec, dv, on ? dv_factor : 0.f);
         }
     }
     fence_before();
@@ -1191,8 +1212,21 @@ bool fits16(const Strided4& t, int64_t dim) {
     return (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && dim % 4 == 0 && t.bs % 4 == 0 && t.ts % 4 == 0 && t.hs % 4 == 0;
 }
 
+// out[i] = sum of `parts` numbers n apart, in order
+__global__ void __launch_bounds__(256) adb_attention_add(const float* part, float* out, int64_t n, int parts) {
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        float s = part[i];
+        for (int p = 1; p < parts; p++) s += part[p * n + i];
+        out[i] = s;
+    }
+}
+cudaError_t add_parts(const float* part, float* out, int64_t n, int64_t parts, CUstream_st* stream) {
+    adb_attention_add<<<unsigned(std::min<int64_t>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(part, out, n, int(parts));
+    return cudaGetLastError();
+}
+
 template <class K, class A>
-cudaError_t launch(K kernel, unsigned grid, int threads, int smem, CUstream_st* stream, const A& args) {
+cudaError_t launch(K kernel, dim3 grid, int threads, int smem, CUstream_st* stream, const A& args) {
     cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     kernel<<<grid, threads, smem, stream>>>(args);
@@ -1200,7 +1234,7 @@ cudaError_t launch(K kernel, unsigned grid, int threads, int smem, CUstream_st* 
 }
 
 template <int P>
-cudaError_t forward(const ForwardArgs& f, unsigned grid, CUstream_st* stream) {
+cudaError_t forward(const ForwardArgs& f, dim3 grid, CUstream_st* stream) {
     constexpr int smem = ForwardShared<P>::BYTES;
     const bool cap = f.a.cap > 0.f, bias = f.a.slopes != nullptr;
     if (cap) return bias ? launch(adb_attention_tc<P, true, true>, grid, THREADS, smem, stream, f) : launch(adb_attention_tc<P, true, false>, grid, THREADS, smem, stream, f);
@@ -1242,7 +1276,7 @@ cudaError_t images(const ImageArgs& im, int jobs, int P, CUstream_st* stream) {
     return cudaGetLastError();
 }
 template <int P, bool KEYS>
-cudaError_t grad_kernel(const GradArgs& f, unsigned grid, CUstream_st* stream) {
+cudaError_t grad_kernel(const GradArgs& f, dim3 grid, CUstream_st* stream) {
     const bool cap = f.a.cap > 0.f, bias = f.a.slopes != nullptr;
     auto go = [&](auto c, auto s) {
         constexpr bool CAP = decltype(c)::value, BIAS = decltype(s)::value;
@@ -1272,6 +1306,7 @@ int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string
     im.job[1] = image_job(cut, a.v, s, true, P);
     if (a.docs) im.job[0].docs = cut.take<float2>(s.batch * tiles);
     cudaError_t e = images(im, 2, P, stream);
+    int n = 2;
     if (e == cudaSuccess) {
         ForwardArgs f{};
         f.a = a;
@@ -1282,10 +1317,17 @@ int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string
         f.q_vec = fits16(a.q, s.dim);
         f.o_vec = aligned_rows(a.o, s.dim);
         f.round = heads_in_round(s, P);
-        const unsigned blocks = unsigned(s.batch * s.heads * ((s.tq + ROWS - 1) / ROWS));
+        const int64_t shares = attention_forward_shares(s, a.sm_count);
+        if (shares > 1) f.partial = cut.take<float>(s.batch * s.tq * s.heads * shares * (s.dim + 2));
+        const dim3 blocks(unsigned(s.batch * s.heads * attention_tc_tiles(s.tq)), unsigned(shares));
         e = P == 1 ? forward<1>(f, blocks, stream) : forward<2>(f, blocks, stream);
+        if (e == cudaSuccess && shares > 1) {
+            attention_join(a, int(shares), f.partial, stream);
+            e = cudaGetLastError();
+            n++;
+        }
     }
-    if (e == cudaSuccess) return 2;
+    if (e == cudaSuccess) return n;
     err = cudaGetErrorString(e);
     return -1;
 }
@@ -1316,16 +1358,33 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
     f.status = a.status;
     f.round = heads_in_round(s, P);
     if (e == cudaSuccess && a.dq) {
-        f.out_vec = aligned_rows(a.dq, s.dim);
-        const unsigned blocks = unsigned(s.batch * s.heads * q_tiles);
+        const int64_t shares = attention_dq_shares(s, a.sm_count), size = s.batch * s.tq * s.heads * s.dim;
+        f.dq = shares > 1 ? cut.take<float>(shares * size) : a.dq;
+        f.out_vec = aligned_rows(f.dq, s.dim);
+        const dim3 blocks(unsigned(s.batch * s.heads * q_tiles), unsigned(shares));
         e = P == 1 ? grad_kernel<1, false>(f, blocks, stream) : grad_kernel<2, false>(f, blocks, stream);
         n++;
+        if (e == cudaSuccess && shares > 1) {
+            e = add_parts(f.dq, a.dq, size, shares, stream);
+            n++;
+        }
     }
     if (e == cudaSuccess && (a.dk || a.dv)) {
-        f.out_vec = aligned_rows(a.dk, s.dim) && aligned_rows(a.dv, s.dim);
-        const unsigned blocks = unsigned(s.batch * s.kv_heads * k_tiles);
+        const int64_t shares = attention_dkv_shares(s, a.sm_count), size = s.batch * s.tk * s.kv_heads * s.dim;
+        auto place = [&](float* out) { return out && shares > 1 ? cut.take<float>(shares * size) : out; };
+        f.dk = place(a.dk);
+        f.dv = place(a.dv);
+        f.out_vec = aligned_rows(f.dk, s.dim) && aligned_rows(f.dv, s.dim);
+        const dim3 blocks(unsigned(s.batch * s.kv_heads * k_tiles), unsigned(shares));
         e = P == 1 ? grad_kernel<1, true>(f, blocks, stream) : grad_kernel<2, true>(f, blocks, stream);
         n++;
+        for (int i = 0; i < 2; i++) {
+            float *part = i ? f.dv : f.dk, *out = i ? a.dv : a.dk;
+            if (e == cudaSuccess && shares > 1 && out) {
+                e = add_parts(part, out, size, shares, stream);
+                n++;
+            }
+        }
     }
     if (e == cudaSuccess) return n;
     err = cudaGetErrorString(e);

@@ -1601,7 +1601,7 @@ class Lowerer {
             }
             return in;
         }, grad ? std::vector<Shape>{qs, ks, ks} : std::vector<Shape>{qs, ls}, {B, Tq, Tk, H, G, D},
-        grad ? attention_grad_workspace(as) : attention_workspace(as, opt_.sm_count));
+        grad ? attention_grad_workspace(as, opt_.sm_count) : attention_workspace(as, opt_.sm_count));
     }
 
     void lower_allreduce(const Cmd& c) {

@@ -76,8 +76,24 @@ struct AttentionArgs {
 constexpr int64_t ATTENTION_TC_MAX_DIM = 128, ATTENTION_TC_TILE = 128;
 constexpr int ATTENTION_GAVE_UP = 33;   // first code of a bounded wait of theirs that ran out
 inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
+// With few queries a tile of 128 is mostly padding and the keys are worth reading once only: adb_attention_decode.cu.
 inline bool attention_uses_tc(const AttentionShape& s) {
-    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 64 && s.tk >= 64 && s.batch * s.heads <= 65535;
+    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 16 && s.tk >= 64 && s.batch * s.heads <= 65535;
+}
+// How many blocks share one tile's walk over the other side when there are fewer tiles than SMs: as many as fill the SMs,
+// each with at least `least` steps.  Their results are added (or joined) in order by a kernel of their own.
+inline int64_t attention_shares(int64_t tiles, int64_t steps, int64_t least, int sm_count) {
+    return std::max<int64_t>(1, std::min(int64_t(sm_count) / tiles, steps / least));
+}
+inline int64_t attention_tc_tiles(int64_t tokens) { return (tokens + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE; }
+inline int64_t attention_forward_shares(const AttentionShape& s, int sm_count) {
+    return attention_shares(s.batch * s.heads * attention_tc_tiles(s.tq), attention_tc_tiles(s.tk), 4, sm_count);
+}
+inline int64_t attention_dq_shares(const AttentionShape& s, int sm_count) {
+    return attention_shares(s.batch * s.heads * attention_tc_tiles(s.tq), 2 * attention_tc_tiles(s.tk), 4, sm_count);
+}
+inline int64_t attention_dkv_shares(const AttentionShape& s, int sm_count) {
+    return attention_shares(s.batch * s.kv_heads * attention_tc_tiles(s.tk), 2 * attention_tc_tiles(s.tq), 4, sm_count);
 }
 // Few queries (adb_attention_decode.cu): the keys are cut into ranges, so that about eight rounds of two blocks per SM
 // have work and a range keeps a block busy for at least one step.
@@ -94,21 +110,23 @@ inline int64_t attention_ranges(const AttentionShape& s, int sm_count) {
 inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
     if (!attention_uses_tc(s)) return s.batch * s.tq * s.heads * attention_ranges(s, sm_count) * (s.dim + 2);
     // images of keys and values, a scale for each, document numbers; each part begins on a 256-byte boundary
-    const int64_t tiles = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, n = s.batch * s.kv_heads * tiles;
-    return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64;
+    const int64_t tiles = attention_tc_tiles(s.tk), n = s.batch * s.kv_heads * tiles, shares = attention_forward_shares(s, sm_count);
+    return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 2 * s.batch * tiles + 64 +
+           (shares > 1 ? s.batch * s.tq * s.heads * shares * (s.dim + 2) : 0);
 }
-// The gradient takes them whatever the count of queries (a tile of 128 is padded): for one query against 60000 keys the
-// CUDA-core kernels, with their 64-row tiles just as empty, need four times as long.
+// The gradient takes them whatever the count of queries: the CUDA-core kernels' tiles of 64 are just as empty.
 inline bool attention_grad_uses_tc(const AttentionShape& s) {
     return s.dim <= ATTENTION_TC_MAX_DIM && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
-inline int64_t attention_grad_workspace(const AttentionShape& s) {
+inline int64_t attention_grad_workspace(const AttentionShape& s, int sm_count) {
     if (!attention_grad_uses_tc(s)) return s.batch * s.heads * s.tq;   // one number per query: the gradient of the output times the output
-    const int64_t kt = (s.tk + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE, qt = (s.tq + ATTENTION_TC_TILE - 1) / ATTENTION_TC_TILE;
+    const int64_t kt = attention_tc_tiles(s.tk), qt = attention_tc_tiles(s.tq);
     const int64_t nk = s.batch * s.kv_heads * kt, nq = s.batch * s.heads * qt;
+    const int64_t q_shares = attention_dq_shares(s, sm_count), k_shares = attention_dkv_shares(s, sm_count);
     // images of four operands with their scales, two norms, logarithms and deltas in whole tiles, document numbers
     return 2 * ((nk + nq) * attention_panels(s.dim) * 8192 + nk + nq + 128) + nk + nq + 128 + 2 * (nq * ATTENTION_TC_TILE + 64) +
-           2 * s.batch * (kt + qt) + 128;
+           2 * s.batch * (kt + qt) + 128 + (q_shares > 1 ? q_shares * s.batch * s.tq * s.heads * s.dim + 64 : 0) +
+           (k_shares > 1 ? 2 * (k_shares * s.batch * s.tk * s.kv_heads * s.dim + 64) : 0);
 }
 
 // Each enqueues its kernels on `stream` and returns how many, or -1 with `err` set.
@@ -117,6 +135,8 @@ int rms_norm_grad_launch(const NormGradArgs& a, CUstream_st* stream, std::string
 int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err);
 int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 int attention_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
+// joins partial[rows][ranges][dim + 2] (unscaled result, maximum, sum) into the output and the logarithms
+void attention_join(const AttentionArgs& a, int ranges, const float* partial, CUstream_st* stream);
 // few queries; 16-byte accesses to keys and values
 int attention_split_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err);
 // where attention_uses_tc
