@@ -26,10 +26,27 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float sum8(float x) {
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    x += __shfl_xor_sync(0xffffffffu, x, 2);
-    return x + __shfl_xor_sync(0xffffffffu, x, 4);
+// Sums of R numbers over eight lanes, each lane left with the one whose row it owns (8 / R lanes own a row together): a lane
+// that gives half of its numbers away at each exchange needs R - 1 + log2(8 / R) of them instead of 3 R, and what follows
+// from a sum (the score, its exponential) is worked out once instead of eight times.
+template <int R> __device__ __forceinline__ int own_row(int l8) { return l8 * R / 8; }
+template <int R>
+__device__ __forceinline__ float own_sum(float (&x)[R], int l8) {
+    int held = R;
+#pragma unroll
+    for (int m = 4; m; m >>= 1) {
+        if (held > 1) {
+            held /= 2;
+#pragma unroll
+            for (int k = 0; k < held; k++) {
+                const bool upper = l8 & m;
+                const float give = upper ? x[k] : x[held + k], keep = upper ? x[held + k] : x[k];
+                x[k] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+            }
+        } else
+            x[0] += __shfl_xor_sync(0xffffffffu, x[0], m);
+    }
+    return x[0];
 }
 
 // 16 bytes, or zeros
@@ -49,10 +66,13 @@ __global__ void __launch_bounds__(THREADS, R * NV <= 16 && NV <= 4 ? 2 : 1) adb_
     __shared__ float sm[WARPS][R], sl[WARPS][R];
     const int dim = int(a.s.dim), heads = int(a.s.heads), kv_heads = int(a.s.kv_heads), group = heads / kv_heads, tq = int(a.s.tq);
     const int rows = group * tq, chunks = (rows + R - 1) / R;
+    // the key heads of the same tokens one after another: their rows lie side by side in memory
     int at = int(blockIdx.x);
-    const int range = at % ranges;
-    at /= ranges;
-    const int chunk = at % chunks, bg = at / chunks, b = bg / kv_heads, g = bg % kv_heads;
+    const int chunk = at % chunks;
+    at /= chunks;
+    const int g = at % kv_heads;
+    at /= kv_heads;
+    const int range = at % ranges, b = at / ranges;
     const Sight sight(a, b);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, l8 = lane % 8, sub = lane / 8;
 
@@ -62,21 +82,17 @@ __global__ void __launch_bounds__(THREADS, R * NV <= 16 && NV <= 4 ? 2 : 1) adb_
         reinterpret_cast<float*>(sq[r])[c] = used ? __ldg(a.q.p + b * a.q.bs + int64_t(i) * a.q.ts + h * a.q.hs + c) : 0.f;
     }
     __syncthreads();
-    int pos[R];
-    float doc[R], m[R], l[R];
-    bool on[R];
+    // the row this lane owns of the R
+    const int row = chunk * R + own_row<R>(l8), pos = row / group + sight.shift;
+    const bool on = row < rows && sight.query_used(pos);
+    const float doc = on && sight.docs ? sight.docs[pos] : 0.f;
+    const ScoreOf score(a, g * group + (row < rows ? row % group : 0));
+    float m = -INFINITY, l = 0.f;
     float4 acc[R][NV];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int row = chunk * R + r;
-        pos[r] = row / group + sight.shift;
-        on[r] = row < rows && sight.query_used(pos[r]);
-        doc[r] = on[r] && sight.docs ? sight.docs[pos[r]] : 0.f;
-        m[r] = -INFINITY;
-        l[r] = 0.f;
+    for (int r = 0; r < R; r++)
 #pragma unroll
         for (int v = 0; v < NV; v++) acc[r][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
     const float *kp = a.k.p + b * a.k.bs + g * a.k.hs + 4 * l8, *vp = a.v.p + b * a.v.bs + g * a.v.hs + 4 * l8;
     const int last_pos = tq - 1 + sight.shift;
     const int end = min(sight.keys_end(last_pos), (range + 1) * range_keys);
@@ -105,14 +121,11 @@ __global__ void __launch_bounds__(THREADS, R * NV <= 16 && NV <= 4 ? 2 : 1) adb_
         asm volatile("cp.async.wait_group 2;" ::: "memory");
         const float4* from = ring + (step % STAGES) * QUADS + threadIdx.x;
         const int j0 = first + step * STEP * GROUPS;
-        bool use[STEP];
+        float dots[STEP][R];
 #pragma unroll
-        for (int u = 0; u < STEP; u++) use[u] = j0 + u * GROUPS < end && sight.key_used(j0 + u * GROUPS);
-        float s[R][STEP];
+        for (int u = 0; u < STEP; u++)
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int u = 0; u < STEP; u++) s[r][u] = 0.f;
+            for (int r = 0; r < R; r++) dots[u][r] = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             float4 x[STEP];
@@ -122,68 +135,66 @@ __global__ void __launch_bounds__(THREADS, R * NV <= 16 && NV <= 4 ? 2 : 1) adb_
             for (int r = 0; r < R; r++) {
                 const float4 q = sq[r][8 * v + l8];
 #pragma unroll
-                for (int u = 0; u < STEP; u++) s[r][u] = fmaf(q.w, x[u].w, fmaf(q.z, x[u].z, fmaf(q.y, x[u].y, fmaf(q.x, x[u].x, s[r][u]))));
+                for (int u = 0; u < STEP; u++) dots[u][r] = fmaf(q.w, x[u].w, fmaf(q.z, x[u].z, fmaf(q.y, x[u].y, fmaf(q.x, x[u].x, dots[u][r]))));
             }
         }
-        float keep[R];
-        bool rises = false;
+        float s[STEP], top = m;
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int row = chunk * R + r;
-            const ScoreOf score(a, g * group + (row < rows ? row % group : 0));
-            float top = m[r];
-#pragma unroll
-            for (int u = 0; u < STEP; u++) {
-                const int j = j0 + u * GROUPS;
-                float bend;
-                const float dot = sum8(s[r][u]);
-                s[r][u] = use[u] && on[r] && sight.sees(pos[r], j, doc[r]) ? score(dot, pos[r], j, bend) : -INFINITY;
-                top = fmaxf(top, s[r][u]);
-            }
-            const float base = top == -INFINITY ? 0.f : top;
-            keep[r] = ex2(m[r] - base);
-            rises = rises || top > m[r];
-            m[r] = top;
-            float sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < STEP; u++) {
-                s[r][u] = ex2(s[r][u] - base);
-                sum += s[r][u];
-            }
-            l[r] = fmaf(l[r], keep[r], sum);
+        for (int u = 0; u < STEP; u++) {
+            const int j = j0 + u * GROUPS;
+            float bend;
+            const float dot = own_sum<R>(dots[u], l8);
+            s[u] = on && j < end && sight.key_used(j) && sight.sees(pos, j, doc) ? score(dot, pos, j, bend) : -INFINITY;
+            top = fmaxf(top, s[u]);
         }
+        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m - base);
         // (a maximum that stays needs no rescaling: every factor is one.  Maxima rise rarely after the first steps.)
-        if (__any_sync(0xffffffffu, rises)) {
+        if (__any_sync(0xffffffffu, top > m)) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int r = 0; r < R; r++) {
+                const float f = __shfl_sync(0xffffffffu, keep, sub * 8 + r * (8 / R));
 #pragma unroll
                 for (int v = 0; v < NV; v++) {
-                    acc[r][v].x *= keep[r]; acc[r][v].y *= keep[r]; acc[r][v].z *= keep[r]; acc[r][v].w *= keep[r];
+                    acc[r][v].x *= f; acc[r][v].y *= f; acc[r][v].z *= f; acc[r][v].w *= f;
                 }
+            }
         }
+        m = top;
+        float sum = 0.f;
 #pragma unroll
-        for (int v = 0; v < NV; v++)
+        for (int u = 0; u < STEP; u++) {
+            s[u] = ex2(s[u] - base);
+            sum += s[u];
+        }
+        l = fmaf(l, keep, sum);
 #pragma unroll
-            for (int u = 0; u < STEP; u++) {
+        for (int u = 0; u < STEP; u++) {
+            float p[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) p[r] = __shfl_sync(0xffffffffu, s[u], sub * 8 + r * (8 / R));
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
                 const float4 x = from[((STEP + u) * NV + v) * THREADS];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    acc[r][v].x = fmaf(s[r][u], x.x, acc[r][v].x);
-                    acc[r][v].y = fmaf(s[r][u], x.y, acc[r][v].y);
-                    acc[r][v].z = fmaf(s[r][u], x.z, acc[r][v].z);
-                    acc[r][v].w = fmaf(s[r][u], x.w, acc[r][v].w);
+                    acc[r][v].x = fmaf(p[r], x.x, acc[r][v].x);
+                    acc[r][v].y = fmaf(p[r], x.y, acc[r][v].y);
+                    acc[r][v].z = fmaf(p[r], x.z, acc[r][v].z);
+                    acc[r][v].w = fmaf(p[r], x.w, acc[r][v].w);
                 }
             }
+        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     // the warp's four groups, then the block's warps
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+        const float mr = __shfl_sync(0xffffffffu, m, sub * 8 + r * (8 / R)), lr = __shfl_sync(0xffffffffu, l, sub * 8 + r * (8 / R));
+        float top = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const float keep = ex2(m[r] - (top == -INFINITY ? 0.f : top));
-        float sum = l[r] * keep;
+        const float keep = ex2(mr - (top == -INFINITY ? 0.f : top));
+        float sum = lr * keep;
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         if (lane == 0) { sm[warp][r] = top; sl[warp][r] = sum; }
