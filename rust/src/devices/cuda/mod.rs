@@ -64,6 +64,7 @@ pub mod flags {
     pub const NO_TINY_DOT: u32 = 4096;
     /// accumulate 1024 instead of 4096 k elements per chunk in the dot kernels: 8e-6 instead of 3e-5 of max|C|, 9 % slower
     pub const SHORT_DOT_CHUNKS: u32 = 8192;
+    pub const DEVICE_RESULTS: u32 = 16384;
 }
 
 pub struct B200 {

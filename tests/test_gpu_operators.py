@@ -94,7 +94,8 @@ def _docs(b, t, size, pad):
 
 
 SIZES = [(1, 1, 1, 1, 1, 1), (2, 64, 64, 2, 2, 64), (1, 65, 65, 3, 1, 40), (2, 127, 129, 4, 2, 128), (1, 200, 333, 2, 2, 80), (1, 50, 70, 2, 1, 160),
-         (1, 33, 40, 2, 2, 256), (2, 130, 260, 4, 1, 6), (1, 513, 513, 2, 1, 96), (1, 300, 1000, 1, 1, 128)]
+         (1, 33, 40, 2, 2, 256), (2, 130, 260, 4, 1, 6), (1, 513, 513, 2, 1, 96), (1, 300, 1000, 1, 1, 128),
+         (2, 17, 300, 4, 2, 64), (1, 63, 64, 2, 2, 128), (1, 700, 1300, 2, 1, 64), (8, 260, 260, 8, 4, 64)]
 
 
 @pytest.mark.parametrize("size", SIZES)
@@ -102,9 +103,9 @@ SIZES = [(1, 1, 1, 1, 1, 1), (2, 64, 64, 2, 2, 64), (1, 65, 65, 3, 1, 40), (2, 1
 def test_attention(size, masks):
     b, tq, tk, h, g, d = size
     kw = {"full": dict(causal=False), "causal": {}, "cap": dict(cap=3.0, slopes=True, causal=False),
-          "docs": dict(docs=_docs(b, tk, 50, 9)), "prefix": dict(prefix=[tk // 3 + 1, 0][:b]),
-          "lengths": dict(lengths=[max(0, tk - 40), tk][:b]),
-          "all": dict(cap=20.0, slopes=True, docs=_docs(b, tk, 90, 20), prefix=[10, tk + 5][:b], lengths=[tk - tk // 5, tk // 2][:b])}[masks]
+          "docs": dict(docs=_docs(b, tk, 50, 9)), "prefix": dict(prefix=([tk // 3 + 1, 0] * b)[:b]),
+          "lengths": dict(lengths=([max(0, tk - 40), tk] * b)[:b]),
+          "all": dict(cap=20.0, slopes=True, docs=_docs(b, tk, 90, 20), prefix=([10, tk + 5] * b)[:b], lengths=([tk - tk // 5, tk // 2] * b)[:b])}[masks]
     c = oc.attention_case(b, tq, tk, h, g, d, seed=tq + d, **kw)
     oc.attention_check(oc.attention_run(b200(), c), c)
 
@@ -307,6 +308,82 @@ def test_eager_captured_and_replayed():
         for x, y in zip(runs[0], r):
             assert np.array_equal(x, y)
     dev.close()
+
+
+@pytest.mark.parametrize("flags", ["FLAG_NO_FUSION", "FLAG_NO_GRAPHS", "FLAG_PROFILE", "FLAG_SERIAL_GRAPHS", "FLAG_DETERMINISTIC"])
+def test_layer_under_flags(flags):
+    dev = adb.devices.B200(0, flags=getattr(adb.devices, flags))
+    got = _train(dev, 2)
+    dev.close()
+    want = _train(oracle(), 2)
+    for n in want:
+        assert np.abs(got[n] - want[n]).max() <= 8e-4 * np.abs(want[n]).max(), n
+
+
+def test_two_handles_at_once():
+    """two programs on two handles of one GPU, executed by two threads at the same time"""
+    import threading
+    cases = [oc.attention_case(2, 400, 400, 4, 2, 64, seed=1), oc.attention_case(2, 300, 500, 4, 4, 128, seed=2, cap=5.0)]
+    devs = [adb.devices.B200(0) for _ in cases]
+    blobs, ids, alive, first = [], [], [], []
+    for dev, c in zip(devs, cases):
+        oc.start(dev)
+        q, k, v = (oc.leaf(c[n]) for n in "qkv")
+        out = ad.attention(q, k, v, cap=c["cap"])
+        loss = out * oc.data(c["do"])
+        loss.forward()
+        loss.backward()
+        kept = dict(out=out.val(), dq=q.grad(), dk=k.grad(), dv=v.grad())
+        for t in kept.values():
+            t.keep()
+        blob, keep = ir.serialize(ad.current_ir(), ad.ret_dep_list())
+        blobs.append(blob)
+        alive.append(keep)
+        ids.append({n: t.id for n, t in kept.items()})
+        dev.execute_blob(blob)
+        first.append({n: dev.get_tensor(t).numpy() for n, t in ids[-1].items()})
+        oc.attention_check(first[-1], c)
+    wrong = []
+
+    def work(i):
+        for _ in range(30):
+            devs[i].execute_blob(blobs[i])
+            if any(not np.array_equal(devs[i].get_tensor(t).numpy(), first[i][n]) for n, t in ids[i].items()):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong
+    for d in devs:
+        d.close()
+
+
+def test_a_decoding_loop():
+    """a cache that grows by a token a step inside one program: lengths are data, the plan stays"""
+    room, d = 200, 64
+    c = oc.attention_case(2, 1, room, 4, 2, d, lengths=[100, 3])
+    oc.start(b200())
+    q, k, v = (oc.data(c[x]) for x in "qkv")
+    total, length = ad.zeros([2, 1, 4, d]), ad.tensor(c["lengths"], [2])
+
+    def step(_):
+        nonlocal total, length
+        total += ad.attention(q, k, v, lengths=length)
+        total.forward()
+        length += np.float32(1.0)
+        length.forward()
+
+    ad.ir_for(range(0, 5), step)
+    got = oc.finish({"total": total.val(), "length": length.val()})
+    want, tol = 0, 0
+    for i in range(5):
+        ref = oc.attention_reference(dict(c, lengths=c["lengths"] + i))["out"]
+        want, tol = want + ref[0], tol + ref[1] + 8 * oc.U * np.abs(ref[0])
+    assert list(got["length"]) == [105, 8]
+    oc.close("total", got["total"], want, tol)
 
 
 def test_results_left_on_the_device():
