@@ -6,8 +6,11 @@
 // up to 8 rows.  Eight lanes read a key together (a lane holds every eighth quad of elements), a warp four keys at once;
 // each group of eight lanes has a running maximum and sum of its own, and groups, warps and ranges meet only at the end.
 // Loads go to shared memory asynchronously, three steps deep, each thread fetching what it will read itself: no barrier,
-// and up to 128 KiB in flight on every SM (with loads into registers, 64 KiB at best and none while a step is computed, the
-// kernel reached 3.4 TB/s).
+// and up to 128 KiB in flight on every SM.
+//
+// Measured, 32 sequences of 8192 to 16384 keys, 32 heads over 8 of 128, 3.2 GB: 475 us, the copy rate.  With loads into
+// registers 960 us; through shared memory, every lane working out every row's scores, 790 us (issue 57 % busy, most of it
+// that); each lane the scores of one row, 475.  One sequence of 1025 keys: 13 us with the joining kernel.
 #include <cuda_runtime.h>
 
 #include "adb_attention.hpp"

@@ -3,6 +3,10 @@
 // The keys and values are first turned into images of 128 rows (adb_attention_images: one read and one write of them, 4 bytes
 // per element each way), so that the kernel proper fetches ready operands by bulk copies however the caller's tensors
 // are strided.
+//
+// Measured on 2 x 4096 tokens, 16 heads of 128, causal (profiles/attention_tc_4096x32x128.md): images 46 us (5.8 TB/s), forward
+// 389 us, images of the gradient's four operands 111 us, dq 686 us, dk and dv 908 us; at the tensor cores' own rate the
+// products take 190, 285 and 380 us.  Error against 64 bits 8e-7 of a result's norm; fp32 products in cuBLAS: 1.7e-6.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -16,8 +20,8 @@ namespace {
 using namespace tc16;
 
 constexpr int KT = 128;                 // keys of a tile
-// Warps that do the arithmetic between the products: PARTS threads a row, each with a share of its columns.  Four of them
-// rather than two (which have registers to spare) hide the latency of tensor memory, exponentials and barriers better.
+// Warps that do the arithmetic between the products: PARTS threads a row, each with a share of its columns.
+// (8 warps instead of 16: dk and dv 1204 us instead of 988, its code too long for the instruction cache.)
 constexpr int PARTS = 4;
 constexpr int SOFTMAX_WARPS = 4 * PARTS, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);

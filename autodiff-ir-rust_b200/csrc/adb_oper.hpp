@@ -26,9 +26,9 @@ struct NormGradArgs {
 constexpr int64_t NORM_GRAD_ONE_PASS = 16384;   // widest row whose share stays in a thread's registers
 // blocks of the gradient kernel: each adds its rows' part of dscale in registers and writes one row of partial sums
 inline int64_t norm_grad_blocks(int64_t rows, int64_t width, int sm_count) {
-    const int64_t rows_per_block = width <= 1024 ? 8 : width <= 2048 ? 2 : 1;
+    const int64_t rows_per_block = width <= 1024 ? 8 : 1;
     const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
-    return std::min<int64_t>(blocks, int64_t(sm_count) * (width <= 4096 ? 2 : 1));
+    return std::min<int64_t>(blocks, int64_t(sm_count) * (width <= 1024 ? 2 : width <= 2048 ? 4 : width <= 4096 ? 2 : 1));
 }
 inline int64_t norm_grad_workspace(int64_t rows, int64_t width, int sm_count) {
     if (width > NORM_GRAD_ONE_PASS) return rows + width * std::min<int64_t>(rows, 64);

@@ -10,7 +10,8 @@
 // and only its distance from a whole number of turns is kept, so that sine and cosine are good to about 2e-7 up to
 // positions of 2^24.
 //
-// Bound by HBM: 8 bytes per element.  A block takes a few tokens: their sines and cosines go into shared memory once and
+// Bound by HBM: 8 bytes per element; 4 x 4096 tokens of 32 heads of 128, 537 MB, take 94 us = 5.7 TB/s, 0.87 of the copy rate.
+// A block takes a few tokens: their sines and cosines go into shared memory once and
 // serve every head.
 #include <cuda_runtime.h>
 
