@@ -39,7 +39,7 @@ struct ImageJob {
     uint8_t* image;
     float* scale;     // [batch * heads][tiles]
     float* norm;      // largest Euclidean norm of a tile's rows, or null
-    float2* docs;     // [batch][tiles]: smallest and largest document number of a tile, or null
+    float4* docs;     // [batch][tiles]: smallest and largest document number of a tile, and whether all of its tokens are used; or null
     // for queries, in rows padded to whole tiles: the logarithm lse (+inf where a query sees nothing, so that its weights
     // vanish), and the gradient of the output times the output
     float *lse, *delta;
@@ -56,7 +56,7 @@ template <int P>
 __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(const ImageArgs args) {
     constexpr int LPR = 16 * P, RPW = 32 / LPR, RUN = ROWS / IMAGE_WARPS, N = RUN / RPW;   // lanes of a row, rows a warp reads at a time, rows of a warp, times
     __shared__ float most[IMAGE_WARPS], longest[IMAGE_WARPS];
-    __shared__ int doc_lo, doc_hi;
+    __shared__ int doc_lo, doc_hi, doc_gaps;
     const ImageJob& job = args.job[blockIdx.z];
     const int tile = blockIdx.x, bh = blockIdx.y;
     if (tile >= job.tiles || bh >= args.a.s.batch * job.heads) return;
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) most[warp] = top;
-    if (threadIdx.x == 0) { doc_lo = 0x7fffffff; doc_hi = -1; }
+    if (threadIdx.x == 0) { doc_lo = 0x7fffffff; doc_hi = -1; doc_gaps = 0; }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < IMAGE_WARPS; w++) top = fmaxf(top, most[w]);
@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
             const int d = __float_as_int(sight.docs[at] + 0.f);   // numbers that are not negative order like their bits
             atomicMin(&doc_lo, d);
             atomicMax(&doc_hi, d);
-        }
+        } else
+            doc_gaps = 1;
     }
     if (!job.norm && !ranges) return;
     __syncthreads();
@@ -154,24 +155,32 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
         for (int w = 0; w < IMAGE_WARPS; w++) l = fmaxf(l, longest[w]);
         job.norm[int64_t(bh) * job.tiles + tile] = sqrtf(l) * scale;
     }
-    if (ranges) job.docs[int64_t(b) * job.tiles + tile] = doc_hi < 0 ? make_float2(INFINITY, -1.f) : make_float2(__int_as_float(doc_lo), __int_as_float(doc_hi));
+    if (ranges)
+        job.docs[int64_t(b) * job.tiles + tile] =
+            doc_hi < 0 ? make_float4(INFINITY, -1.f, 0.f, 0.f) : make_float4(__int_as_float(doc_lo), __int_as_float(doc_hi), doc_gaps ? 0.f : 1.f, 0.f);
 }
 
 // ------------------------------------------------------------------------------------------ which tiles of the other side count
 struct Walk {
     int begin, end;              // tiles
-    const float2* range;         // document numbers of runs of 128 tokens, or null
+    const float4* range;         // document numbers of runs of 128 tokens, or null
     float lo, hi;                // this block's
     int halves;                  // 1: tiles are 64 tokens, half a run
     __device__ __forceinline__ int from(int t) const {
         for (; t < end; t++) {
             if (!range) return t;
-            const float2 r = __ldg(range + (t >> halves));
+            const float4 r = __ldg(range + (t >> halves));
             if (r.x <= hi && r.y >= lo) return t;
         }
         return -1;
     }
     __device__ __forceinline__ int first() const { return from(begin); }
+    // documents hide nothing between this block and tile t: all of both lie in one
+    __device__ __forceinline__ bool one_document(int t) const {
+        if (!range) return true;
+        const float4 r = __ldg(range + (t >> halves));
+        return r.z != 0.f && r.x == r.y && lo == hi && r.x == lo;
+    }
     // what block blockIdx.y of gridDim.y takes of the walk
     __device__ __forceinline__ void share() {
         const int n = max(end - begin, 0), at = begin;
@@ -314,7 +323,7 @@ struct ForwardArgs {
     AttentionArgs a;
     const uint8_t *k, *v;
     const float *k_scale, *v_scale;
-    const float2* doc_range;
+    const float4* doc_range;
     int* status;
     int q_vec, o_vec, round;
     float* partial;   // of blocks that share a tile
@@ -484,12 +493,15 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         int i = 0;
         const int pos_first = q0 + sight.shift;
         int t = walk.first();
+        bool docs_next = t >= 0 && !walk.one_document(t);
         float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
         for (int next; t >= 0; t = next, i++) {
             const int k0 = t * KT + KEYS * part;
             const float mul = q_scale * k_next * score.mul, v_scale = v_next;
+            const bool by_docs = docs_next;
             next = walk.from(t + 1);
             if (next >= 0) {   // a tile ahead: a load takes longer than the waits below should
+                docs_next = !walk.one_document(next);
                 k_next = __ldg(f.k_scale + image0 + next);
                 v_next = __ldg(f.v_scale + image0 + next);
             }
@@ -515,12 +527,12 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 for (int c = 0; c < KEYS; c++) s[c] = fmaf(-slope2, fabsf(away - float(c)), s[c]);
             }
             const int k_last = k0 + KEYS - 1;
-            if (k_last >= sight.n || sight.docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
+            if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
                 // keys from `ahead` on are hidden by the length or the order
                 const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
 #pragma unroll
                 for (int c = 0; c < KEYS; c++)
-                    if (c >= ahead || (sight.docs && __ldg(sight.docs + k0 + c) != doc)) s[c] = -INFINITY;
+                    if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) s[c] = -INFINITY;
             }
             float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -699,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
     walk.share();
     walk.range = sight.docs ? f.k.docs + int64_t(b) * k_tiles : nullptr;
     if (sight.docs) {
-        const float2 own = __ldg(f.q.docs + int64_t(b) * q_tiles + q0 / ROWS);
+        const float4 own = __ldg(f.q.docs + int64_t(b) * q_tiles + q0 / ROWS);
         walk.lo = own.x;
         walk.hi = own.y;
     }
@@ -818,12 +830,15 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         };
         const int pos_first = q0 + sight.shift;
         int t = walk.first();
+        bool docs_next = t >= 0 && !walk.one_document(t);
         float k_next = t >= 0 ? __ldg(f.k.scale + image0 + (t >> 1)) : 0.f, v_next = t >= 0 ? __ldg(f.v.scale + image0 + (t >> 1)) : 0.f;
         for (int next; t >= 0; t = next, n++) {
             const int k0 = t * GT + KEYS * part;
             const float k_scale = k_next, v_scale = v_next;
+            const bool by_docs = docs_next;
             next = walk.from(t + 1);
             if (next >= 0) {   // a tile ahead
+                docs_next = !walk.one_document(next);
                 k_next = __ldg(f.k.scale + image0 + (next >> 1));
                 v_next = __ldg(f.v.scale + image0 + (next >> 1));
             }
@@ -849,11 +864,11 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                 p[c] = ex2(s - lse);
             }
             const int k_last = k0 + KEYS - 1;
-            if (k_last >= sight.n || sight.docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
+            if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
                 const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
 #pragma unroll
                 for (int c = 0; c < KEYS; c++)
-                    if (c >= ahead || (sight.docs && __ldg(sight.docs + k0 + c) != doc)) p[c] = 0.f;
+                    if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) p[c] = 0.f;
             }
             if (n > 0) ok = drain(n - 1);     // beside the product dP
             if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
@@ -996,7 +1011,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     walk.share();
     walk.range = sight.docs ? f.q.docs + int64_t(b) * q_tiles : nullptr;
     if (sight.docs) {
-        const float2 own = __ldg(f.k.docs + int64_t(b) * k_tiles + tile);
+        const float4 own = __ldg(f.k.docs + int64_t(b) * k_tiles + tile);
         walk.lo = own.x;
         walk.hi = own.y;
     }
@@ -1120,10 +1135,12 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             return true;
         };
         float q_next = 0.f, o_next = 0.f, slope_next = 0.f;
+        bool docs_next = false;
         auto look = [&]() {   // what belongs to the tile of queries that `at` stands on
             const int64_t image = (head0 + at.head) * q_tiles + (at.t >> 1);
             q_next = __ldg(f.q.scale + image);
             o_next = __ldg(f.dout.scale + image);
+            docs_next = !walk.one_document(at.t);
             if constexpr (BIAS) slope_next = __ldg(a.slopes + g * group + at.head) * LOG2E;
         };
         if (any) look();
@@ -1131,6 +1148,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         for (bool more = any; more; n++) {
             const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
             const float q_scale = q_next, o_scale = o_next, slope2 = slope_next;
+            const bool by_docs = docs_next;
             more = at.next();
             if (more) look();   // a tile ahead
             const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale, ds_mul = ds_factor * (q_scale / most_q), p_mul = 1024.f * (o_scale / most_o);
@@ -1138,7 +1156,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             fence_after();
             const float4* lse = reinterpret_cast<const float4*>(gen + stats(n)) + QUERIES / 4 * part;
             const float4* delta = lse + GT / 4;
-            const bool partly = sight.docs || (sight.causal && q0 + sight.shift < k0 + ROWS - 1 && k0 + ROWS - 1 >= sight.prefix);
+            const bool partly = by_docs || (sight.causal && q0 + sight.shift < k0 + ROWS - 1 && k0 + ROWS - 1 >= sight.prefix);
             const int behind = sight.causal && j >= sight.prefix ? j - sight.shift - q0 : 0;   // queries in front of the key
             static_assert(QUERIES == 16, "a thread's columns of a tile");
             float p[QUERIES];      // weights, times the scores' bend once they are stored
@@ -1163,7 +1181,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                         float w = ex2(s - l4[e]);
                         if (partly) {
                             const int q = q0 + c + e;
-                            if (c + e < behind || (sight.docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
+                            if (c + e < behind || (by_docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
                         }
                         x[c + e] = w * p_mul;
                         p[c + e] = CAP ? w * bend : w;
@@ -1308,7 +1326,7 @@ int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string
     im.a = a;
     im.job[0] = image_job(cut, a.k, s, true, P);
     im.job[1] = image_job(cut, a.v, s, true, P);
-    if (a.docs) im.job[0].docs = cut.take<float2>(s.batch * tiles);
+    if (a.docs) im.job[0].docs = cut.take<float4>(s.batch * tiles);
     cudaError_t e = images(im, 2, P, stream);
     int n = 2;
     if (e == cudaSuccess) {
@@ -1351,8 +1369,8 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
     im.job[2].lse = cut.take<float>(s.batch * s.heads * q_tiles * ROWS);
     im.job[3].delta = cut.take<float>(s.batch * s.heads * q_tiles * ROWS);
     if (a.docs) {
-        im.job[0].docs = cut.take<float2>(s.batch * k_tiles);
-        im.job[2].docs = cut.take<float2>(s.batch * q_tiles);
+        im.job[0].docs = cut.take<float4>(s.batch * k_tiles);
+        im.job[2].docs = cut.take<float4>(s.batch * q_tiles);
     }
     cudaError_t e = images(im, 4, P, stream);
     int n = 1;
