@@ -171,7 +171,7 @@ struct adb_device {
         std::vector<uint64_t> dims;
         float* host = nullptr;      // pinned, cached across calls
         size_t host_cap = 0;
-        const float* dev = nullptr;
+        const float* dev = nullptr; // null once an execute has begun that reuses the memory
         size_t n = 0;
         bool valid = false;
         bool fetched = false;
@@ -1052,6 +1052,12 @@ float* pinned_alloc(adb_device* d, size_t bytes, size_t& cap) {
     return p;
 }
 
+void drop_results(adb_device* d) {
+    for (auto& r : d->results)
+        if (r.host && r.host_cap) d->pinned_pool.push_back({r.host, r.host_cap});
+    d->results.clear();
+}
+
 adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
     auto t_begin = std::chrono::steady_clock::now();
     Program prog = parse_program(blob, nbytes);
@@ -1137,6 +1143,13 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
     d->stats.plan_steps = uint64_t(plan.n_steps);
     d->stats.arena_bytes = uint64_t(plan.arena_bytes);
 
+    // From here on the memory that the last execute's results lie in is freed or written over.  When this execute fails, what
+    // had been copied to the host can still be had, the rest cannot.
+    for (auto& r : d->results) {
+        r.dev = nullptr;
+        if (!r.fetched) r.valid = false;
+    }
+
     // arena
     if (size_t(plan.arena_bytes) > d->arena_cap) {
         if (d->arena) ck(cudaFree(d->arena), "cudaFree(arena)");
@@ -1179,10 +1192,12 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
     ck(cudaEventRecord(ev1, d->stream), "event record");
 
     // read-back of dep-list ids (src/devices/opencl/device.rs:82-87)
-    for (auto& r : d->results) {
-        if (r.host && r.host_cap) d->pinned_pool.push_back({r.host, r.host_cap});
-    }
-    d->results.clear();
+    drop_results(d);
+    struct ResultGuard {   // results count once the device has finished without an error
+        adb_device* d;
+        bool complete = false;
+        ~ResultGuard() { if (!complete) drop_results(d); }
+    } result_guard{d};
     // small kept tensors sit side by side at the start of the arena: one copy brings all of them back
     float* block = nullptr;
     const bool leave = (d->flags & ADB_FLAG_DEVICE_RESULTS) != 0;
@@ -1228,6 +1243,7 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
         d->err = std::string(gs >= ATTENTION_GAVE_UP ? "attention" : "tensor-core dot product") + " gave up on a bounded wait (code " + std::to_string(gs) + "); results are invalid";
         return ADB_ERR_CUDA;
     }
+    result_guard.complete = true;
     float ms_run = 0, ms_rb = 0;
     ck(cudaEventElapsedTime(&ms_run, ev0, ev1), "elapsed time");
     ck(cudaEventElapsedTime(&ms_rb, ev1, ev2), "elapsed time");
@@ -1443,7 +1459,7 @@ adb_status adb_get_tensor_device(adb_device* d, const char* id, const float** dp
     if (!d || !id) return ADB_ERR_INVALID;
     for (auto& r : d->results)
         if (r.id == id) {
-            if (!r.valid) return ADB_NONE;
+            if (!r.valid || (!r.dev && r.n)) return ADB_NONE;
             if (dptr) *dptr = r.dev;
             if (dims) *dims = r.dims.data();
             if (ndim) *ndim = uint32_t(r.dims.size());

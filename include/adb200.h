@@ -138,7 +138,9 @@ typedef struct adb_config {
 
 #define ADB_FLAG_DEVICE_RESULTS 16384u  /* adb_execute leaves the kept tensors in HBM: adb_get_tensor copies one when it is asked for
                                          it, adb_get_tensor_device as without the flag (by default every kept tensor is
-                                         copied to the host inside adb_execute, as the reference does) */
+                                         copied to the host inside adb_execute, as the reference does).  A tensor that
+                                         was not asked for is gone once the next adb_execute has begun to run, even
+                                         when that one fails: ADB_NONE */
 
 /* Replaces OpenCL::new (src/devices/opencl/device.rs:41-58) + autodiff::set_device's device slot
  * (src/core/autodiff.rs:82-97).  Fails with ADB_ERR_NO_DEVICE when no GPU is present. */
@@ -159,7 +161,8 @@ adb_status adb_get_tensor(adb_device *dev, const char *id, const float **data,
                           const uint64_t **dims, uint32_t *ndim);
 
 /* Like adb_get_tensor but leaves the data in HBM: *dptr is the device address of the id's buffer
- * (valid until the next adb_execute).  No reference counterpart (the reference always copies back). */
+ * (valid until the next adb_execute; ADB_NONE once one has begun to run, even when that one fails).
+ * No reference counterpart (the reference always copies back). */
 adb_status adb_get_tensor_device(adb_device *dev, const char *id, const float **dptr,
                                  const uint64_t **dims, uint32_t *ndim);
 
