@@ -1221,7 +1221,9 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
             hr.n = size_t(numel(ri.shape));
             hr.dev = ex.buf_ptr(ri.buf, ri.off);
             const BufferInfo& bi = plan.bufs[size_t(ri.buf)];
-            if (leave) {
+            // payload memory is only borrowed for the duration of the call: what a kept id finds there is copied at once
+            const bool stays = leave && !bi.external;
+            if (stays) {
                 // copied when adb_get_tensor asks for it
             } else if (block && !bi.external && bi.arena_off >= 0 && bi.arena_off + (ri.off + int64_t(hr.n)) * 4 <= plan.results_bytes) {
                 hr.host = block + bi.arena_off / 4 + ri.off;   // inside the shared block: not returned to the pool
@@ -1231,7 +1233,7 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
                 if (hr.n) ck(cudaMemcpyAsync(hr.host, hr.dev, hr.n * 4, cudaMemcpyDeviceToHost, d->stream), "read-back");
                 d->stats.d2h_bytes += hr.n * 4;
             }
-            hr.fetched = !leave;
+            hr.fetched = !stays;
         }
         d->results.push_back(std::move(hr));
     }

@@ -140,7 +140,8 @@ typedef struct adb_config {
                                          it, adb_get_tensor_device as without the flag (by default every kept tensor is
                                          copied to the host inside adb_execute, as the reference does).  A tensor that
                                          was not asked for is gone once the next adb_execute has begun to run, even
-                                         when that one fails: ADB_NONE */
+                                         when that one fails: ADB_NONE.  A kept id that is bound to a device payload is
+                                         copied inside adb_execute all the same, as that memory is borrowed */
 
 /* Replaces OpenCL::new (src/devices/opencl/device.rs:41-58) + autodiff::set_device's device slot
  * (src/core/autodiff.rs:82-97).  Fails with ADB_ERR_NO_DEVICE when no GPU is present. */

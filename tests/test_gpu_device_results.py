@@ -71,3 +71,21 @@ def test_host_copies_outlive_an_execute_that_found_no_memory():
     assert np.array_equal(d.get_tensor(e).numpy().reshape(-1), 3 * b)
     assert d.get_tensor_device(e) is None
     d.close()
+
+
+def test_a_kept_payload_of_the_callers_is_read_before_execute_returns(dev):
+    """device payloads are borrowed for the duration of execute: a kept id that is bound to one holds what was there then"""
+    torch = pytest.importorskip("torch")
+    x = torch.arange(1000.0, device="cuda")
+    torch.cuda.synchronize()
+    oc.start(dev)
+    a = ad.tensor(ir.DevicePayload(x.data_ptr(), x.numel(), x), [10, 100])
+    y = a * 3.0
+    a.forward().keep()
+    y.forward().keep()
+    ad.execute()
+    x.fill_(-1.0)
+    torch.cuda.synchronize()
+    want = np.arange(1000, dtype=np.float32)
+    assert np.array_equal(a.val().get().numpy().reshape(-1), want)
+    assert np.array_equal(y.val().get().numpy().reshape(-1), 3 * want)
