@@ -973,6 +973,8 @@ def rotary(x: Tensor, table: Tensor, positions: Tensor = None, offset: int = 0, 
         raise ValueError("rotary: positions and an offset exclude one another")
     if abs(offset) > 1 << 24 or int(offset) != offset:
         raise ValueError("rotary: the offset must be a whole number within 2^24")
+    if positions is None and offset + d[1] - 1 > 1 << 24:
+        raise ValueError("rotary: the last token's position is beyond 2^24")
     return Tensor(OperatorNode(_Rotary([x, table, positions], [int(bool(interleaved)), 0, int(offset)], [float(gain)])))
 
 

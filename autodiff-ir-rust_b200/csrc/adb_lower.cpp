@@ -1535,7 +1535,10 @@ class Lowerer {
         if (pos && pos->shape != Shape{s[1]} && pos->shape != Shape{s[0], s[1]}) fail("Rotary: positions must be [tokens] or [batch, tokens]");
         for (int k = 0; k < 2; k++)
             if (c.ints[size_t(k)] != 0 && c.ints[size_t(k)] != 1) fail("Rotary: a flag that is neither 0 nor 1");
-        if (c.ints[2] < -(int64_t(1) << 24) || c.ints[2] > (int64_t(1) << 24)) fail("Rotary: the first position is beyond 2^24");
+        // positions are floats in the kernel; beyond 2^24 some whole numbers are none
+        const int64_t most = int64_t(1) << 24;
+        if (c.ints[2] < -most || c.ints[2] > most) fail("Rotary: the first position is beyond 2^24");
+        if (!pos && s[1] > 0 && s[1] - 1 > most - c.ints[2]) fail("Rotary: the last position is beyond 2^24");
         if (numel(s) == 0) {
             consume_args(c);
             bind_result(c, 0, 0.f, s);

@@ -71,7 +71,8 @@ typedef enum adb_status {
  *     32 Rotary        x[B,T,H,D] table[2,P] [positions [T] or [B,T]] -> y; ints: interleaved, inverse, offset;
  *                      reals: gain.  The first 2 P elements of every head, taken in pairs (2i, 2i+1) or (i, P+i), are
  *                      turned by position * (table[0][i] + table[1][i]) whole turns (backwards with `inverse`) and
- *                      multiplied by gain; without positions token t stands at offset + t.  P <= 4096, |offset| <= 2^24.
+ *                      multiplied by gain; without positions token t stands at offset + t.  P <= 4096, |offset| <= 2^24,
+ *                      offset + T - 1 <= 2^24 (every whole number up to there is a float).
  *     33 Attention     q[B,Tq,H,D] k v[B,Tk,G,D] [slopes [H]] [documents [B,Tk]] [prefix [B]] [lengths [B]]
  *                      -> out[B,Tq,H,D] lse[B,H,Tq] (base 2); ints: causal; reals: scale, cap (0: none)
  *                      1 <= D <= 256, H a multiple of G, fewer than 2^24 tokens, Tq <= Tk with documents, prefix only with causal.

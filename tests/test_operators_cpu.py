@@ -334,3 +334,28 @@ def test_mixed_distribution_is_refused():
     blob, alive = ir.serialize(ad.current_ir(), {y.val().id, z.val().id})
     with pytest.raises(adb.devices.AdbError, match="rows"):
         adb.devices.shard_ir(blob, 0, 2, 4)
+
+
+@pytest.mark.parametrize("offset,tokens,good", [((1 << 24) - 2, 3, True), ((1 << 24) - 2, 4, False), (1 << 24, 1, True), (1 << 24, 2, False),
+                                                (-(1 << 24), 2, True), (-(1 << 24) - 1, 2, False)])
+def test_positions_end_where_floats_are_whole_numbers(offset, tokens, good):
+    """beyond 2^24 a position would round to a neighbour's"""
+    oc.start(OracleDevice())
+    x, t = _zeros(1, tokens, 1, 4), _mat("t", 2, 2)
+    cmds = [_mat("x", 1, tokens, 1, 4), t, ("Rotary", ["x", "t", None], ["y"], [0, 0, offset], [1.0])]
+    if good:
+        ad.rotary(x, _zeros(2, 2), offset=offset)
+        _lower(cmds, ["y"])
+        return
+    with pytest.raises(ValueError, match="24"):
+        ad.rotary(x, _zeros(2, 2), offset=offset)
+    with pytest.raises(adb.devices.AdbError, match="24"):
+        _lower(cmds, ["y"])
+
+
+def test_more_tokens_than_positions_are_refused():
+    """2^24 + 2 tokens counted from 0: the last one's position is no float"""
+    oc.start(OracleDevice())
+    x = _zeros(1, 1, 1, 2).broadcast(1, (1 << 24) + 2)
+    with pytest.raises(ValueError, match="24"):
+        ad.rotary(x, _zeros(2, 1))
