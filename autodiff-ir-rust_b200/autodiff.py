@@ -237,6 +237,8 @@ class Tensor:
         finally:
             _State.passes -= 1
             if not _State.passes:
+                for op in _State.waiting.values():   # the pass raised: the next one starts afresh
+                    op.grads = None
                 _State.waiting.clear()
 
     def dim(self) -> list:

@@ -359,3 +359,29 @@ def test_more_tokens_than_positions_are_refused():
     x = _zeros(1, 1, 1, 2).broadcast(1, (1 << 24) + 2)
     with pytest.raises(ValueError, match="24"):
         ad.rotary(x, _zeros(2, 1))
+
+
+def test_a_backward_pass_that_raised_leaves_no_gradients_behind():
+    class Bad(ad.Node):
+        def __init__(self, t): self.t = t
+        def forward(self): return self.t.forward()
+        def backward(self, grad): raise RuntimeError("no gradient")
+        def dim(self): return self.t.dim()
+        def val(self): return self.t.val()
+
+    dev = OracleDevice()
+    oc.start(dev)
+    w = oc.leaf(np.ones((1, 2, 1, 4)))
+    y = nn.Rotary(4).f(w)
+    loss = y + ad.Tensor(Bad(oc.leaf(np.ones((1, 2, 1, 4)))))
+    loss.forward()
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    again = y * 3.0
+    again.forward()
+    again.backward()
+    g = w.grad()
+    g.keep()
+    ad.execute()
+    want = oc.rotary_reference(np.ones((1, 2, 1, 4)), np.full((1, 2, 1, 4), 3.0), 4)["dx"]
+    oc.close("dw", np.asarray(g.get().data).reshape(1, 2, 1, 4), *want)
