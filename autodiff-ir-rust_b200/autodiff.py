@@ -1008,7 +1008,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, scale: float = None, causal: bool
     prefix   [batch]: the first keys of a sequence, which every query sees in spite of the causal mask
     lengths  [batch]: how many keys of the cache a sequence has; the rest is not read
 
-    A query that sees nothing gives zeros.  No gradient flows into slopes, docs, prefix and lengths."""
+    On the device, heads of up to 128 elements run on the tensor cores, with operands as sums of two halves; a device made
+    with FLAG_SIMT_DOT keeps to fp32 products.  A query that sees nothing gives zeros.  No gradient flows into slopes, docs, prefix and lengths."""
     dq, dk = q.dim(), k.dim()
     if len(dq) != 4 or len(dk) != 4 or v.dim() != dk:
         raise ValueError(f"attention: operands {dq}, {dk}, {v.dim()} are not [batch, tokens, heads, size]")

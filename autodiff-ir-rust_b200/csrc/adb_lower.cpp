@@ -1594,7 +1594,7 @@ class Lowerer {
                 bind_result(c, 1, -std::numeric_limits<float>::infinity(), ls);
             return;
         }
-        const AttentionShape as{B, Tq, Tk, H, G, D};
+        const AttentionShape as{B, Tq, Tk, H, G, D, opt_.simt_dot};
         push_oper(c, [&] {
             std::vector<Access> in;
             for (size_t i = 0; i < c.args.size(); i++) {

@@ -52,6 +52,7 @@ struct RotaryArgs {
 constexpr int64_t ATTENTION_MAX_DIM = 256;
 struct AttentionShape {
     int64_t batch = 0, tq = 0, tk = 0, heads = 0, kv_heads = 0, dim = 0;
+    bool cuda_cores = false;   // fp32 products only (ADB_FLAG_SIMT_DOT)
 };
 struct Strided4 {   // [batch, tokens, heads, dim], dim contiguous
     const float* p = nullptr;
@@ -80,7 +81,7 @@ inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
 // 8 queries on the tile is the faster one all the same (8 queries of 16 heads over 4 against 8000 keys: 50 us against 94;
 // 15 of 32 heads over 32 against 2000: 59 against 90).
 inline bool attention_uses_tc(const AttentionShape& s) {
-    return s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 8 && s.tk >= 64 && s.batch * s.heads <= 65535;
+    return !s.cuda_cores && s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 8 && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
 // How many blocks share one tile's walk over the other side when there are fewer tiles than SMs: as many as fill the SMs,
 // each with at least `least` steps.  Their results are added (or joined) in order by a kernel of their own.
@@ -118,7 +119,7 @@ inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
 }
 // The gradient takes them whatever the count of queries: the CUDA-core kernels' tiles of 64 are just as empty.
 inline bool attention_grad_uses_tc(const AttentionShape& s) {
-    return s.dim <= ATTENTION_TC_MAX_DIM && s.tk >= 64 && s.batch * s.heads <= 65535;
+    return !s.cuda_cores && s.dim <= ATTENTION_TC_MAX_DIM && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
 inline int64_t attention_grad_workspace(const AttentionShape& s, int sm_count) {
     if (!attention_grad_uses_tc(s)) return s.batch * s.heads * s.tq;   // one number per query: the gradient of the output times the output

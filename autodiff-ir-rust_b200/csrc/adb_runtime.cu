@@ -514,7 +514,7 @@ class Executor {
                 return Strided4{in(i), x.stride[0], x.stride[1], x.stride[2]};
             };
             AttentionArgs a;
-            a.s = {o.dims[0], o.dims[1], o.dims[2], o.dims[3], o.dims[4], o.dims[5]};
+            a.s = {o.dims[0], o.dims[1], o.dims[2], o.dims[3], o.dims[4], o.dims[5], (d_->flags & ADB_FLAG_SIMT_DOT) != 0};
             a.q = four(0); a.k = four(1); a.v = four(2);
             a.slopes = in(3); a.docs = in(4); a.prefix = in(5); a.lengths = in(6);
             a.causal = int(o.ints[0]);
@@ -1110,6 +1110,7 @@ adb_status do_execute(adb_device* d, const uint8_t* blob, size_t nbytes) {
         opt.exact_div = (d->flags & ADB_FLAG_EXACT_DIV) != 0;
         opt.fuse_small_sums = (d->flags & ADB_FLAG_FUSE_SMALL_SUMS) != 0;
         opt.no_grouping = (d->flags & ADB_FLAG_NO_GROUPING) != 0;
+        opt.simt_dot = (d->flags & ADB_FLAG_SIMT_DOT) != 0;
         opt.no_tiny_dot = (d->flags & ADB_FLAG_NO_TINY_DOT) != 0;
         opt.bucket_collectives = d->world > 1 && !(d->flags & (ADB_FLAG_COMM_STREAM | ADB_FLAG_NO_BUCKETS));
         opt.rank = d->rank;
@@ -1512,6 +1513,7 @@ adb_status adb_lower_check(const uint8_t* blob, size_t nbytes, const adb_config*
             opt.exact_div = (cfg->flags & ADB_FLAG_EXACT_DIV) != 0;
             opt.fuse_small_sums = (cfg->flags & ADB_FLAG_FUSE_SMALL_SUMS) != 0;
             opt.no_grouping = (cfg->flags & ADB_FLAG_NO_GROUPING) != 0;
+            opt.simt_dot = (cfg->flags & ADB_FLAG_SIMT_DOT) != 0;
             opt.no_tiny_dot = (cfg->flags & ADB_FLAG_NO_TINY_DOT) != 0;
             opt.bucket_collectives = cfg->world_size > 1 && !(cfg->flags & (ADB_FLAG_COMM_STREAM | ADB_FLAG_NO_BUCKETS));
             opt.rank = cfg->rank;

@@ -105,7 +105,9 @@ typedef struct adb_config {
 
 #define ADB_FLAG_NO_GRAPHS 1u         /* launch loop bodies kernel by kernel instead of replaying CUDA graphs */
 #define ADB_FLAG_NO_FUSION 2u         /* one kernel per IR command (debug aid, like the reference's unfused path) */
-#define ADB_FLAG_SIMT_DOT 4u          /* force the plain fp32 dot kernel instead of the tcgen05 3xTF32 kernels */
+#define ADB_FLAG_SIMT_DOT 4u          /* force the plain fp32 dot kernel instead of the tcgen05 3xTF32 kernels, and
+                                         attention's fp32 kernels on the CUDA cores instead of those that make fp32
+                                         products of fp16 halves on the tensor cores */
 #define ADB_FLAG_PROFILE 8u           /* CUDA events around every kernel (fills the per-kind times of adb_stats);
                                          loop bodies are then launched kernel by kernel, not as graphs */
 #define ADB_FLAG_COMM_STREAM 16u      /* issue collectives on a second, high-priority stream (ordered by events on the
