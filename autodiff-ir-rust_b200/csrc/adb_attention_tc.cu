@@ -25,7 +25,9 @@ constexpr int KT = 128;                 // keys of a tile
 constexpr int PARTS = 4;
 constexpr int SOFTMAX_WARPS = 4 * PARTS, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
-constexpr float P_SHIFT = 10.f;         // weights are kept 2^10 times as large: a weight of 2^-24 still has 20 bits
+// Weights of a tile are kept in units that make the row's largest 2^15: half of fp16's smallest step, 2^-25, is 2^-40 of it,
+// and a weight of 2^-18 of the row's largest still has both halves' 22 bits.
+constexpr float P_SHIFT = 15.f;
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -38,7 +40,6 @@ struct ImageJob {
     Strided4 src;
     uint8_t* image;
     float* scale;     // [batch * heads][tiles]
-    float* norm;      // largest Euclidean norm of a tile's rows, or null
     float4* docs;     // [batch][tiles]: smallest and largest document number of a tile, and whether all of its tokens are used; or null
     // for queries, in rows padded to whole tiles: the logarithm lse (+inf where a query sees nothing, so that its weights
     // vanish), and the gradient of the output times the output
@@ -55,7 +56,7 @@ constexpr int IMAGE_WARPS = 16;
 template <int P>
 __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(const ImageArgs args) {
     constexpr int LPR = 16 * P, RPW = 32 / LPR, RUN = ROWS / IMAGE_WARPS, N = RUN / RPW;   // lanes of a row, rows a warp reads at a time, rows of a warp, times
-    __shared__ float most[IMAGE_WARPS], longest[IMAGE_WARPS];
+    __shared__ float most[IMAGE_WARPS];
     __shared__ int doc_lo, doc_hi, doc_gaps;
     const ImageJob& job = args.job[blockIdx.z];
     const int tile = blockIdx.x, bh = blockIdx.y;
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
     const Sight sight(args.a, b);
     const float* src = job.src.p + b * job.src.bs + h * job.src.hs;
     float4 v[N];
-    float top = 0.f, len = 0.f;
+    float top = 0.f;
     auto quad = [&](const float* p, bool vec) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (vec) {
@@ -124,18 +125,8 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
         const int at = (c / 64) * PANEL_BYTES + row * 128 + ((((c % 64) / 8) ^ (row & 7)) * 16) + (c % 8) * 2;
         *reinterpret_cast<uint2*>(image + at) = hi;
         *reinterpret_cast<uint2*>(image + P * PANEL_BYTES + at) = lo;
-        if (job.norm) {
-            float s = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
-#pragma unroll
-            for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            len = fmaxf(len, s);
-        }
     }
     if (threadIdx.x == 0) job.scale[int64_t(bh) * job.tiles + tile] = scale;
-    if (job.norm) {
-        if (RPW > 1) len = fmaxf(len, __shfl_xor_sync(0xffffffffu, len, 16));
-        if (lane == 0) longest[warp] = len;
-    }
     const bool ranges = job.docs && h == 0;
     if (ranges && threadIdx.x < ROWS) {
         const int t = tile * ROWS + threadIdx.x, at = job.of_keys ? t : t + sight.shift;
@@ -146,16 +137,9 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
         } else
             doc_gaps = 1;
     }
-    if (!job.norm && !ranges) return;
+    if (!ranges) return;
     __syncthreads();
-    if (threadIdx.x) return;
-    if (job.norm) {
-        float l = 0.f;
-#pragma unroll
-        for (int w = 0; w < IMAGE_WARPS; w++) l = fmaxf(l, longest[w]);
-        job.norm[int64_t(bh) * job.tiles + tile] = sqrtf(l) * scale;
-    }
-    if (ranges)
+    if (threadIdx.x == 0)
         job.docs[int64_t(b) * job.tiles + tile] =
             doc_hi < 0 ? make_float4(INFINITY, -1.f, 0.f, 0.f) : make_float4(__int_as_float(doc_lo), __int_as_float(doc_hi), doc_gaps ? 0.f : 1.f, 0.f);
 }
@@ -202,7 +186,7 @@ int heads_in_round(const AttentionShape& s, int P) {
     return int(std::max<int64_t>(1, std::min(n, most)));
 }
 
-enum : int { GAVE_UP_Q = ATTENTION_GAVE_UP, GAVE_UP_SLOT, GAVE_UP_DATA, GAVE_UP_S, GAVE_UP_P, GAVE_UP_O_FULL, GAVE_UP_O_EMPTY };
+enum : int { GAVE_UP_Q = ATTENTION_GAVE_UP, GAVE_UP_SLOT, GAVE_UP_DATA, GAVE_UP_S, GAVE_UP_P, GAVE_UP_O_FULL, GAVE_UP_O_EMPTY, GAVE_UP_MEET };
 
 // a thread's share of a row as fp32, zero outside
 template <int N>
@@ -544,9 +528,10 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
 #pragma unroll
             for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
             if (!ok) break;
-            const float top = fmaxf(m, row_max(cell, row));
-            const float from = (top == -INFINITY ? 0.f : top) - P_SHIFT;
-            const float fade = ex2(m - from - P_SHIFT);
+            // weights in units of the tile's own largest, sums and results in units of the largest so far
+            const float tile_top = row_max(cell, row), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
+            const float from = (tile_top == -INFINITY ? 0.f : tile_top) - P_SHIFT;
+            const float fade = ex2(m - base), unit = ex2(tile_top - base - P_SHIFT);
             m = top;
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -559,10 +544,10 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_ready(i & 1));
-            l = fmaf(l, fade, (sums[0] + sums[1]) + (sums[2] + sums[3]));
+            l = fmaf(l, fade, ((sums[0] + sums[1]) + (sums[2] + sums[3])) * unit);
             if (i > 0) ok = drain(i - 1);
             keep = fade;
-            v_before = v_scale;
+            v_before = v_scale * unit;
         }
         if (ok && i > 0) ok = drain(i - 1);
         float* cell = exchange + (i & 1) * PARTS * ROWS;   // (the last tile's may still be being read)
@@ -579,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
                     store_row_part<SHARE>(p, part * SHARE, dim, false, acc, 1.f);
                     if (part == 0) {
-                        p[dim] = any ? m - P_SHIFT : -INFINITY;
+                        p[dim] = any ? m : -INFINITY;
                         p[dim + 1] = any ? l : 0.f;
                     }
                 } else if (a.o) {
@@ -588,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
                     store_row_part<SHARE>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
                 }
-                if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + (log2f(l) - P_SHIFT) : -INFINITY;
+                if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + log2f(l) : -INFINITY;
             }
         }
     }
@@ -602,11 +587,12 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
 // Seven products where five would do: the scores and the weights' gradients are formed once in a kernel that owns queries
 // (dq) and once in one that owns keys (dk, dv), so that every sum has one owner, nothing is added by atomics of several
 // blocks and a gradient has the same bits in every run.  The other side passes by in tiles of 64 tokens, two roles fetch and
-// multiply and eight warps do the arithmetic between the products, as in the forward kernel.
+// multiply and 16 warps do the arithmetic between the products, as in the forward kernel.
 //
-// What goes back into tensor memory as an operand is scaled into fp16's range by powers of two: weights by 2^10, the
-// scores' gradients by a bound, |ds| <= scale * (|do_i| |v_j| + |delta_i|) with norms taken from the images.  The images of a
-// side have a scale for each 128 rows; a sum over several of them is kept in units of the largest.
+// What goes back into tensor memory as an operand (weights and the scores' gradients) is divided by a power of two that the
+// row's four threads agree on for every tile, from the largest magnitude among the 64 that they hold; the factor comes back
+// when the accumulator is emptied into registers, as does the scale of the passing tile's image.  So the error of a
+// gradient is a fraction of what it is made of, whatever the size of rows that it does not see.
 // Accumulators are emptied into registers after every tile: each addition in tensor memory truncates, by 2^-24 of the sum
 // so far on average and always towards zero, and the first keys of a causal sequence get their largest terms first
 // (emptied every 8 tiles, dk and dv of 1500 tokens were off by 2.5e-6, against 1e-6 for fp32 sums).
@@ -628,13 +614,21 @@ __device__ __forceinline__ void fetch_half_image(uint32_t dst, const uint8_t* im
 #pragma unroll
     for (int i = 0; i < 2 * P; i++) bulk_load(dst + i * SUB_BYTES, src + i * PANEL_BYTES, SUB_BYTES, bar);
 }
-// largest of n positive numbers, the block's threads together (cell: a shared word set to 0 before)
-__device__ __forceinline__ void block_max(int* cell, const float* p, int n) {
-    float m = 0.f;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) m = fmaxf(m, __ldg(p + i));
+// The largest of what a row's four threads hold, exchanged through shared memory: meeting `count` of the quadrant's warps.
+// (A barrier with a bounded wait: a warp that gave up does not come.  Two meetings in turn use different cells: a cell is
+// written again only after the meeting between, to which everybody came after reading it.)
+template <int N>
+__device__ __forceinline__ bool row_largest(const float (&x)[N], float* exchange, uint32_t meet, uint32_t count, int part, int row, volatile int* stop, int* status, float& most) {
+    float* cell = exchange + (count & 1) * PARTS * ROWS;
+    float top = 0.f;   // (an infinity may set the unit: it reaches every element of the row's sum anyway)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) atomicMax(cell, __float_as_int(m));
+    for (int c = 0; c < N; c++) top = fmaxf(top, fabsf(x[c]));
+    cell[part * ROWS + row] = top;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(meet);
+    if (!bar_wait_warp(meet, count & 1, stop, status, GAVE_UP_MEET)) return false;
+    most = row_max(cell, row);
+    return true;
 }
 
 // dq.  Tensor memory (P panels): Q and dO 64 P columns each, dq 64 P, S 64, dP 64 (over which ds is written).
@@ -644,8 +638,8 @@ template <int P>
 struct QueryGradShared {
     static constexpr int SLOTS = 3;   // of keys and of values
     static constexpr int SLOT_BYTES = 2 * P * SUB_BYTES;
-    static constexpr int BARS = 4 * SLOTS + 7;
-    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + PARTS * ROWS * 4 + BARS * 8 + 32;
+    static constexpr int BARS = 4 * SLOTS + 11;
+    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16;
 };
 
 template <int P, bool CAP, bool BIAS>
@@ -656,8 +650,8 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    float* exchange = reinterpret_cast<float*>(gen + 2 * SLOTS * SLOT);   // [PARTS][128]
-    const uint32_t bars = base + 2 * SLOTS * SLOT + PARTS * ROWS * 4;
+    float* exchange = reinterpret_cast<float*>(gen + 2 * SLOTS * SLOT);   // [2][PARTS][128]
+    const uint32_t bars = base + 2 * SLOTS * SLOT + 2 * PARTS * ROWS * 4;
     auto k_slot = [&](uint32_t n) { return base + (n % SLOTS) * SLOT; };
     auto v_slot = [&](uint32_t n) { return base + (SLOTS + n % SLOTS) * SLOT; };
     auto k_full = [&](uint32_t n) { return bars + 8u * (n % SLOTS); };
@@ -665,10 +659,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
     auto v_full = [&](uint32_t n) { return bars + 8u * (2 * SLOTS + n % SLOTS); };
     auto v_empty = [&](uint32_t n) { return bars + 8u * (3 * SLOTS + n % SLOTS); };
     const uint32_t own_ready = bars + 8u * (4 * SLOTS), s_full = own_ready + 8, s_taken = own_ready + 16, dp_full = own_ready + 24,
-                   ds_ready = own_ready + 32, acc_full = own_ready + 40, acc_taken = own_ready + 48;
+                   ds_ready = own_ready + 32, acc_full = own_ready + 40, acc_taken = own_ready + 48, meet = own_ready + 56;   // meet: one for each quadrant
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (bars - base) + Shared::BARS * 8);
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* cells = const_cast<int*>(reinterpret_cast<volatile int*>(tmem_slot + 2));      // document span [2], largest scale, largest norm
 
     const AttentionArgs& a = f.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -690,16 +683,11 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         bar_init(ds_ready, SOFTMAX_WARPS);
         bar_init(acc_full, 1);
         bar_init(acc_taken, SOFTMAX_WARPS);
+        for (int i = 0; i < 4; i++) bar_init(meet + 8 * i, PARTS);
         *stop = 0;
-        cells[0] = 0x7fffffff;
-        cells[1] = -1;
-        cells[2] = cells[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
-    __syncthreads();
-    block_max(&cells[2], f.k.scale + image0, (keys_end + ROWS - 1) / ROWS);
-    block_max(&cells[3], f.v.norm + image0, (keys_end + ROWS - 1) / ROWS);
     fence_before();
     __syncthreads();
     fence_after();
@@ -781,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         const bool on = q < tq && sight.query_used(pos);
         const float doc = on && sight.docs ? sight.docs[pos] : 0.f;
         const float lse = f.q.lse[int64_t(bh) * q_tiles * ROWS + q], delta = f.dout.delta[int64_t(bh) * q_tiles * ROWS + q];
-        float own_scale[2], length = 0.f;
+        float own_scale[2];
 #pragma unroll
         for (int which = 0; which < 2; which++) {
             const Strided4& src = which ? a.dout : a.q;
@@ -790,27 +778,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             exchange[part * ROWS + row] = largest(x);
             row_sync(quad);
             own_scale[which] = tile_scale(row_max(exchange, row));
-            const float inv = 1.f / own_scale[which];
             const uint32_t column = which ? C_DO : C_Q;
-            store_halves<SHARE>(lanes + column + part * SHARE, x, inv);
+            store_halves<SHARE>(lanes + column + part * SHARE, x, 1.f / own_scale[which]);
             row_sync(quad);
-            if (which) {
-#pragma unroll
-                for (int c = 0; c < SHARE; c++) length = fmaf(x[c] * inv, x[c] * inv, length);
-                exchange[part * ROWS + row] = length;
-                row_sync(quad);
-                length = sqrtf(row_sum(exchange, row)) * own_scale[1];
-            }
         }
         tmem_wait_store();
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(own_ready);
         const ScoreOf score(a, h);
-        const float most_k = __int_as_float(cells[2]), most_v = __int_as_float(cells[3]);
-        const float unit = tile_scale(fabsf(a.scale) * fmaf(length, most_v, fabsf(delta)));   // of ds
-        const float ds_factor = a.scale / unit, out_factor = unit * most_k;
-        float acc[SHARE];
+        float acc[SHARE], factor = 0.f;   // of the accumulator that has not been emptied yet
 #pragma unroll
         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
         bool ok = true;
@@ -825,7 +802,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             __syncwarp();
             if (lane == 0) bar_arrive(acc_taken);
 #pragma unroll
-            for (int c = 0; c < SHARE; c++) acc[c] += __uint_as_float(r[c]);
+            for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), factor, acc[c]);
             return true;
         };
         const int pos_first = q0 + sight.shift;
@@ -842,8 +819,8 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                 k_next = __ldg(f.k.scale + image0 + (next >> 1));
                 v_next = __ldg(f.v.scale + image0 + (next >> 1));
             }
-            const float mul = own_scale[0] * k_scale * score.mul, dp_mul = own_scale[1] * v_scale, ds_mul = ds_factor * (k_scale / most_k);
-            float p[KEYS], bend[CAP ? KEYS : 1];
+            const float mul = own_scale[0] * k_scale * score.mul, dp_mul = own_scale[1] * v_scale;
+            float p[KEYS];   // weights, times the scores' bend
             uint32_t r[KEYS];
             if (!bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
@@ -854,14 +831,14 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             if (lane == 0) bar_arrive(s_taken);
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
-                float s = __uint_as_float(r[c]) * mul;
+                float s = __uint_as_float(r[c]) * mul, bend = 1.f;
                 if constexpr (CAP) {
                     const float w = tanh_exact(s);
-                    bend[c] = fmaf(-w, w, 1.f);
+                    bend = fmaf(-w, w, 1.f);
                     s = score.cap2 * w;
                 }
                 if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(pos - k0 - c)), s);
-                p[c] = ex2(s - lse);
+                p[c] = CAP ? ex2(s - lse) * bend : ex2(s - lse);
             }
             const int k_last = k0 + KEYS - 1;
             if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
@@ -877,11 +854,13 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             tmem_wait_load();
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
-                float w = fmaf(__uint_as_float(r[c]), dp_mul, -delta) * ds_mul;
-                if constexpr (CAP) w *= bend[c];
-                p[c] = p[c] == 0.f ? 0.f : p[c] * w;
+                p[c] = p[c] == 0.f ? 0.f : p[c] * fmaf(__uint_as_float(r[c]), dp_mul, -delta);
             }
-            store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f);
+            float most;
+            if (!row_largest(p, exchange, meet + 8 * quad, n, part, row, stop, f.status, most)) { ok = false; break; }
+            const float unit = tile_scale(most);
+            factor = unit * k_scale * a.scale;
+            store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f / unit);
             tmem_wait_store();
             fence_before();
             __syncwarp();
@@ -892,7 +871,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             if (!on)
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, on ? out_factor : 0.f);
+            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, 1.f);
         }
     }
     fence_before();
@@ -912,8 +891,8 @@ struct KeyGradShared {
     static constexpr int DATA_BYTES = 2 * P * SUB_BYTES;
     static constexpr int STATS_BYTES = 2 * GT * 4;
     static constexpr int OWN_BYTES = P == 2 ? image_bytes(P) : 0;
-    static constexpr int BARS = 4 * SLOTS + 10;
-    static constexpr int BYTES = 1024 + OWN_BYTES + 2 * SLOTS * DATA_BYTES + SLOTS * STATS_BYTES + BARS * 8 + 32;
+    static constexpr int BARS = 4 * SLOTS + 14;
+    static constexpr int BYTES = 1024 + OWN_BYTES + 2 * SLOTS * DATA_BYTES + SLOTS * STATS_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16;
 };
 
 // the tiles of queries of one head after another
@@ -951,8 +930,10 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    constexpr int AT_DATA = Shared::OWN_BYTES, AT_STATS = AT_DATA + 2 * SLOTS * DATA, AT_BARS = AT_STATS + SLOTS * STATS;
+    constexpr int AT_DATA = Shared::OWN_BYTES, AT_STATS = AT_DATA + 2 * SLOTS * DATA, AT_EXCHANGE = AT_STATS + SLOTS * STATS,
+                  AT_BARS = AT_EXCHANGE + 2 * PARTS * ROWS * 4;
     const uint32_t bars = base + AT_BARS;
+    float* exchange = reinterpret_cast<float*>(gen + AT_EXCHANGE);   // [2][PARTS][128]
     auto q_slot = [&](uint32_t n) { return base + AT_DATA + (n % SLOTS) * DATA; };
     auto o_slot = [&](uint32_t n) { return base + AT_DATA + (SLOTS + n % SLOTS) * DATA; };
     auto stats = [&](uint32_t n) { return AT_STATS + int(n % SLOTS) * STATS; };
@@ -962,10 +943,9 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     auto o_empty = [&](uint32_t n) { return bars + 8u * (3 * SLOTS + n % SLOTS); };
     const uint32_t own_ready = bars + 8u * (4 * SLOTS), own_landed = own_ready + 8, s_full = own_ready + 16, p_ready = own_ready + 24,
                    dp_full = own_ready + 32, ds_ready = own_ready + 40, dv_full = own_ready + 48, dv_taken = own_ready + 56, dk_full = own_ready + 64,
-                   dk_taken = own_ready + 72;
+                   dk_taken = own_ready + 72, meet = own_ready + 80;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + AT_BARS + Shared::BARS * 8);
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* cells = const_cast<int*>(reinterpret_cast<volatile int*>(tmem_slot + 2));   // largest scale of q and of do, norm of do and of v
 
     const AttentionArgs& a = f.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -990,16 +970,11 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         bar_init(dv_taken, SOFTMAX_WARPS);
         bar_init(dk_full, 1);
         bar_init(dk_taken, SOFTMAX_WARPS);
+        for (int i = 0; i < 4; i++) bar_init(meet + 8 * i, PARTS);
         *stop = 0;
-        cells[0] = cells[1] = cells[2] = cells[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
-    __syncthreads();
-    block_max(&cells[0], f.q.scale + head0 * q_tiles, group * q_tiles);
-    block_max(&cells[1], f.dout.scale + head0 * q_tiles, group * q_tiles);
-    block_max(&cells[2], f.dout.norm + head0 * q_tiles, group * q_tiles);
-    block_max(&cells[3], f.v.norm + int64_t(bg) * k_tiles, k_tiles);
     fence_before();
     __syncthreads();
     fence_after();
@@ -1108,17 +1083,13 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(own_ready);
-        const float most_q = __int_as_float(cells[0]), most_o = __int_as_float(cells[1]), norm_o = __int_as_float(cells[2]), norm_v = __int_as_float(cells[3]);
-        const float unit = tile_scale(fabsf(a.scale) * norm_o * (__ldg(f.v.norm + own_image) + norm_v));   // of ds
-        const float ds_factor = a.scale / unit, dk_factor = unit * most_q;
-        const float dv_factor = most_o * (1.f / 1024.f);
         const int64_t out_row = (((int64_t(blockIdx.y) * a.s.batch + b) * tk + j) * kv_heads + g) * dim;
         bool ok = true;
         uint32_t n = 0;
-        float dk[SHARE], dv[SHARE];
+        float dk[SHARE], dv[SHARE], dk_factor = 0.f, dv_factor = 0.f;   // factors: of the accumulators that have not been emptied yet
 #pragma unroll
         for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
-        auto drain = [&](uint32_t full, uint32_t taken, uint32_t column, uint32_t tile, float (&acc)[SHARE]) {
+        auto drain = [&](uint32_t full, uint32_t taken, uint32_t column, uint32_t tile, float (&acc)[SHARE], float factor) {
             if (!bar_wait_warp(full, tile & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
             fence_after();
 #pragma unroll
@@ -1127,7 +1098,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                 tmem_load(lanes + column + part * SHARE + c, r);
                 tmem_wait_load();
 #pragma unroll
-                for (int k = 0; k < 16; k++) acc[c + k] += __uint_as_float(r[k]);
+                for (int k = 0; k < 16; k++) acc[c + k] = fmaf(__uint_as_float(r[k]), factor, acc[c + k]);
             }
             fence_before();
             __syncwarp();
@@ -1151,7 +1122,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             const bool by_docs = docs_next;
             more = at.next();
             if (more) look();   // a tile ahead
-            const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale, ds_mul = ds_factor * (q_scale / most_q), p_mul = 1024.f * (o_scale / most_o);
+            const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale;
             if (!ok || !bar_wait_warp(q_full(n), (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA) || !bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
             const float4* lse = reinterpret_cast<const float4*>(gen + stats(n)) + QUERIES / 4 * part;
@@ -1159,10 +1130,9 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             const bool partly = by_docs || (sight.causal && q0 + sight.shift < k0 + ROWS - 1 && k0 + ROWS - 1 >= sight.prefix);
             const int behind = sight.causal && j >= sight.prefix ? j - sight.shift - q0 : 0;   // queries in front of the key
             static_assert(QUERIES == 16, "a thread's columns of a tile");
-            float p[QUERIES];      // weights, times the scores' bend once they are stored
+            float p[QUERIES], bends[CAP ? QUERIES : 1], most;   // weights, and the scores' bend
             uint32_t r[QUERIES];
             {
-                float x[QUERIES];
                 tmem_load(lanes + C_S + QUERIES * part, r);
                 tmem_wait_load();
 #pragma unroll
@@ -1171,10 +1141,10 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                     const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float s = __uint_as_float(r[c + e]) * mul, bend = 1.f;
+                        float s = __uint_as_float(r[c + e]) * mul;
                         if constexpr (CAP) {
                             const float w = tanh_exact(s);
-                            bend = fmaf(-w, w, 1.f);
+                            bends[c + e] = fmaf(-w, w, 1.f);
                             s = score.cap2 * w;
                         }
                         if constexpr (BIAS) s = fmaf(-slope2, fabsf(float(q0 + c + e + sight.shift - j)), s);
@@ -1183,17 +1153,22 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                             const int q = q0 + c + e;
                             if (c + e < behind || (by_docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
                         }
-                        x[c + e] = w * p_mul;
-                        p[c + e] = CAP ? w * bend : w;
+                        p[c + e] = w;
                     }
                 }
-                store_halves<QUERIES>(lanes + C_S + QUERIES * part, x, 1.f);
+                if (!row_largest(p, exchange, meet + 8 * quad, 2 * n, part, row, stop, f.status, most)) { ok = false; break; }
+                const float unit = tile_scale(most);
+                dv_factor = unit * o_scale;
+                store_halves<QUERIES>(lanes + C_S + QUERIES * part, p, 1.f / unit);
             }
+            if constexpr (CAP)
+#pragma unroll
+                for (int c = 0; c < QUERIES; c++) p[c] *= bends[c];
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_ready);
-            if (n > 0) ok = drain(dk_full, dk_taken, C_DK, n - 1, dk);   // beside the product dP
+            if (n > 0) ok = drain(dk_full, dk_taken, C_DK, n - 1, dk, dk_factor);   // beside the product dP
             if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
             tmem_load(lanes + C_DP + QUERIES * part, r);
@@ -1204,24 +1179,26 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                 const float d4[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float w = fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]) * ds_mul;
-                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * w;
+                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]);
                 }
             }
-            store_halves<QUERIES>(lanes + C_DP + QUERIES * part, p, 1.f);
+            if (!row_largest(p, exchange, meet + 8 * quad, 2 * n + 1, part, row, stop, f.status, most)) { ok = false; break; }
+            const float unit = tile_scale(most);
+            dk_factor = unit * q_scale * a.scale;
+            store_halves<QUERIES>(lanes + C_DP + QUERIES * part, p, 1.f / unit);
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(ds_ready);
-            ok = drain(dv_full, dv_taken, C_DV, n, dv);                  // beside the product S
+            ok = drain(dv_full, dv_taken, C_DV, n, dv, dv_factor);                  // beside the product S
         }
-        if (ok && n > 0) ok = drain(dk_full, dk_taken, C_DK, n - 1, dk);
+        if (ok && n > 0) ok = drain(dk_full, dk_taken, C_DK, n - 1, dk, dk_factor);
         if (ok && j < tk) {
             if (!on)   // no query sees the key, whatever its row was compared with
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
-            if (f.dk) store_row_part<SHARE>(f.dk + out_row, part * SHARE, dim, f.out_vec, dk, on ? dk_factor : 0.f);
-            if (f.dv) store_row_part<SHARE>(f.dv + out_row, part * SHARE, dim, f.out_vec, dv, on ? dv_factor : 0.f);
+            if (f.dk) store_row_part<SHARE>(f.dk + out_row, part * SHARE, dim, f.out_vec, dk, 1.f);
+            if (f.dv) store_row_part<SHARE>(f.dv + out_row, part * SHARE, dim, f.out_vec, dv, 1.f);
         }
     }
     fence_before();
@@ -1364,8 +1341,6 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
     const Strided4* const src[4] = {&a.k, &a.v, &a.q, &a.dout};
     for (int i = 0; i < 4; i++) im.job[i] = image_job(cut, *src[i], s, i < 2, P);
     const int k_tiles = im.job[0].tiles, q_tiles = im.job[2].tiles;
-    im.job[1].norm = cut.take<float>(s.batch * s.kv_heads * k_tiles);
-    im.job[3].norm = cut.take<float>(s.batch * s.heads * q_tiles);
     im.job[2].lse = cut.take<float>(s.batch * s.heads * q_tiles * ROWS);
     im.job[3].delta = cut.take<float>(s.batch * s.heads * q_tiles * ROWS);
     if (a.docs) {

@@ -126,8 +126,8 @@ inline int64_t attention_grad_workspace(const AttentionShape& s, int sm_count) {
     const int64_t kt = attention_tc_tiles(s.tk), qt = attention_tc_tiles(s.tq);
     const int64_t nk = s.batch * s.kv_heads * kt, nq = s.batch * s.heads * qt;
     const int64_t q_shares = attention_dq_shares(s, sm_count), k_shares = attention_dkv_shares(s, sm_count);
-    // images of four operands with their scales, two norms, logarithms and deltas in whole tiles, document numbers
-    return 2 * ((nk + nq) * attention_panels(s.dim) * 8192 + nk + nq + 128) + nk + nq + 128 + 2 * (nq * ATTENTION_TC_TILE + 64) +
+    // images of four operands with their scales, logarithms and deltas in whole tiles, document numbers
+    return 2 * ((nk + nq) * attention_panels(s.dim) * 8192 + nk + nq + 128) + 2 * (nq * ATTENTION_TC_TILE + 64) +
            4 * s.batch * (kt + qt) + 128 + (q_shares > 1 ? q_shares * s.batch * s.tq * s.heads * s.dim + 64 : 0) +
            (k_shares > 1 ? 2 * (k_shares * s.batch * s.tk * s.kv_heads * s.dim + 64) : 0);
 }

@@ -37,3 +37,51 @@ def test_fp32_products_on_request(no_floors, d, ratio):
     few = dict(c, **{n: c[n][:, -12:] for n in ("q", "do")})
     oc.attention_check(oc.attention_run(dev, few, grad=False), few)
     dev.close()
+
+
+def _tc_and_fp32(c, **kw):
+    for flags in (0, adb.devices.FLAG_SIMT_DOT):
+        dev = adb.devices.B200(0, flags=flags)
+        oc.attention_check(oc.attention_run(dev, c, **kw), c)
+        dev.close()
+
+
+@pytest.mark.parametrize("d,heads", [(64, 4), (128, 2), (80, 2)])
+@pytest.mark.parametrize("ratio", [2.0 ** -10, 2.0 ** -20, 2.0 ** -50])
+def test_documents_that_fill_tiles_of_their_own(no_floors, d, heads, ratio):
+    """a document's results do not depend on the size of another document's tokens in the same row"""
+    tokens = 1000
+    docs = np.tile(np.arange(tokens) // 256, (1, 1))
+    c = oc.attention_case(1, tokens, tokens, heads, heads // 2, d, seed=3, docs=docs)
+    small = (docs[0] % 2).astype(bool)
+    for n, f in (("q", 1 / ratio), ("k", ratio), ("v", ratio), ("do", ratio)):
+        c[n][:, small] *= np.float32(f)
+    _tc_and_fp32(c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_in_front_of_a_key_do_not_set_its_units(no_floors, d):
+    """under the causal mask the first 512 tokens' large gradients do not reach the keys behind them"""
+    c = oc.attention_case(1, 1024, 1024, 2, 2, d, seed=5)
+    c["do"][:, :512] *= np.float32(2.0 ** 40)
+    _tc_and_fp32(c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("few", [False, True])
+def test_keys_of_little_weight(no_floors, d, few):
+    """keys whose weight is 2^-60 everywhere: small gradients, not zero or rounded ones; with them alone in a tile, too"""
+    c = oc.attention_case(1, 300, 300, 2, 2, d, seed=6, scale=1.0, causal=False)
+    c["q"][..., 0], c["k"][..., 0] = 1.0, 0.0
+    c["q"][..., 1:] *= np.float32(1 / np.sqrt(d))
+    at = [7, 130, 200] if few else np.arange(128, 256)
+    c["k"][:, at, :, 0] = np.float32(-60 * np.log(2))
+    ref = oc.attention_reference(c)
+    # a query's gradients are held in halves in units of the row's largest: its first element, which these keys alone
+    # make up, is as exact as the row's others are
+    ref["dq"] = ref["dq"][0], np.broadcast_to(ref["dq"][1].max(-1, keepdims=True), ref["dq"][0].shape)
+    for flags in (0, adb.devices.FLAG_SIMT_DOT):
+        dev = adb.devices.B200(0, flags=flags)
+        for n, x in oc.attention_run(dev, c).items():
+            oc.close(n, x, *ref[n])
+        dev.close()
