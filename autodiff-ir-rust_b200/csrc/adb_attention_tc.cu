@@ -39,7 +39,9 @@ __device__ __forceinline__ float ex2(float x) {
 struct ImageJob {
     Strided4 src;
     uint8_t* image;
-    float* scale;     // [batch * heads][tiles]
+    // Units of the image: one for a tile whose rows are of similar size, [batch * heads][tiles], negative where every row
+    // has its own; and, in any case, row by row in whole tiles, [batch * heads][tiles * 128].
+    float *scale, *rows;
     float4* docs;     // [batch][tiles]: smallest and largest document number of a tile, and whether all of its tokens are used; or null
     // for queries, in rows padded to whole tiles: the logarithm lse (+inf where a query sees nothing, so that its weights
     // vanish), and the gradient of the output times the output
@@ -52,11 +54,14 @@ struct ImageArgs {
 };
 
 constexpr int IMAGE_WARPS = 16;
+// Rows share a unit when none but rows of zeros has its largest magnitude below 2^-10 of the tile's: half of fp16's
+// smallest step is then at most 2^-29 of any row's largest, 1/32 of half an fp32 step of it.
+constexpr float SIMILAR = 1.f / 1024.f;
 
 template <int P>
 __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(const ImageArgs args) {
     constexpr int LPR = 16 * P, RPW = 32 / LPR, RUN = ROWS / IMAGE_WARPS, N = RUN / RPW;   // lanes of a row, rows a warp reads at a time, rows of a warp, times
-    __shared__ float most[IMAGE_WARPS];
+    __shared__ float most[IMAGE_WARPS], least[IMAGE_WARPS];
     __shared__ int doc_lo, doc_hi, doc_gaps;
     const ImageJob& job = args.job[blockIdx.z];
     const int tile = blockIdx.x, bh = blockIdx.y;
@@ -66,7 +71,7 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
     const Sight sight(args.a, b);
     const float* src = job.src.p + b * job.src.bs + h * job.src.hs;
     float4 v[N];
-    float top = 0.f;
+    float top = 0.f, low = INFINITY;   // of the rows' largest magnitudes
     auto quad = [&](const float* p, bool vec) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (vec) {
@@ -103,21 +108,35 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
             const float x = used(t) ? __ldg(args.a.lse_in + int64_t(bh) * job.tokens + t) : -INFINITY;
             job.lse[padded0 + t] = x == -INFINITY ? INFINITY : x;
         }
+    auto row_top = [&](const float4& x) {
+        float m = fmaxf(fmaxf(finite_magnitude(x.x), finite_magnitude(x.y)), fmaxf(finite_magnitude(x.z), finite_magnitude(x.w)));
 #pragma unroll
-    for (int i = 0; i < N; i++)
-        top = fmaxf(fmaxf(fmaxf(top, finite_magnitude(v[i].x)), finite_magnitude(v[i].y)), fmaxf(finite_magnitude(v[i].z), finite_magnitude(v[i].w)));
+        for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    };
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) most[warp] = top;
+    for (int i = 0; i < N; i++) {
+        const float m = row_top(v[i]);
+        top = fmaxf(top, m);
+        low = fminf(low, m == 0.f ? INFINITY : m);
+    }
+    if (RPW > 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 16));
+    }
+    if (lane == 0) { most[warp] = top; least[warp] = low; }
     if (threadIdx.x == 0) { doc_lo = 0x7fffffff; doc_hi = -1; doc_gaps = 0; }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < IMAGE_WARPS; w++) top = fmaxf(top, most[w]);
-    const float scale = tile_scale(top), inv = 1.f / scale;
+    for (int w = 0; w < IMAGE_WARPS; w++) { top = fmaxf(top, most[w]); low = fminf(low, least[w]); }
+    const bool similar = low >= top * SIMILAR;
+    const float scale = tile_scale(top);
     uint8_t* image = job.image + (int64_t(bh) * job.tiles + tile) * image_bytes(P);
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int row = warp * RUN + i * RPW + lane / LPR;
+        const float own = similar ? scale : tile_scale(row_top(v[i])), inv = 1.f / own;
+        if (lane % LPR == 0) job.rows[padded0 + token(i)] = own;
         uint2 hi, lo;
         const float4 x = make_float4(v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv);
         halves(x.x, x.y, hi.x, lo.x);
@@ -126,7 +145,7 @@ __global__ void __launch_bounds__(32 * IMAGE_WARPS, 2) adb_attention_images(cons
         *reinterpret_cast<uint2*>(image + at) = hi;
         *reinterpret_cast<uint2*>(image + P * PANEL_BYTES + at) = lo;
     }
-    if (threadIdx.x == 0) job.scale[int64_t(bh) * job.tiles + tile] = scale;
+    if (threadIdx.x == 0) job.scale[int64_t(bh) * job.tiles + tile] = similar ? scale : -scale;
     const bool ranges = job.docs && h == 0;
     if (ranges && threadIdx.x < ROWS) {
         const int t = tile * ROWS + threadIdx.x, at = job.of_keys ? t : t + sight.shift;
@@ -235,6 +254,36 @@ __device__ __forceinline__ void store_row_part(float* p, int c0, int dim, bool v
         }
     }
 }
+// Whether some of n tiles of either operand have units by row (each of `threads` threads looks at some of them).  A block
+// then takes the units of all its tiles row by row, in code of its own, so that the usual case does not pay for it.
+__device__ __forceinline__ bool units_by_row(const float* one, const float* other, int n, int thread, int threads) {
+    bool any = false;
+    for (int i = thread; i < n; i += threads) any |= fminf(__ldg(one + i), __ldg(other + i)) < 0.f;   // (both loads at once)
+    return any;
+}
+// a tile's columns times the units of the rows they stand for (16-byte boundary)
+template <int N>
+__device__ __forceinline__ void times_rows(uint32_t (&r)[N], const float* units) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(units + c));
+        const float f[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[c + e] = __float_as_uint(__uint_as_float(r[c + e]) * f[e]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void times_rows(float (&x)[N], const float* units, float factor = 1.f) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(units + c));
+        const float f[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[c + e] *= f[e] * factor;
+    }
+}
+// What a row's unit is multiplied with to give its largest magnitude, within a factor of two.
+constexpr float ROW_TOP = 16384.f;
 // the warps that share a quadrant's rows
 __device__ __forceinline__ void row_sync(int quad) { asm volatile("bar.sync %0, %1;" ::"r"(1 + quad), "n"(32 * PARTS) : "memory"); }
 // largest, or sum, of what the row's threads put down
@@ -306,7 +355,7 @@ __device__ __forceinline__ void rows_mma(uint32_t e, uint32_t d, uint32_t a, uin
 struct ForwardArgs {
     AttentionArgs a;
     const uint8_t *k, *v;
-    const float *k_scale, *v_scale;
+    const float *k_scale, *v_scale, *k_rows, *v_rows;
     const float4* doc_range;
     int* status;
     int q_vec, o_vec, round;
@@ -318,7 +367,7 @@ struct ForwardShared {
     static constexpr int SLOTS = P == 2 ? 3 : 6;
     static constexpr int SLOT_BYTES = image_bytes(P);
     static constexpr int BARS = 2 * SLOTS + 7;
-    static constexpr int BYTES = 1024 + SLOTS * SLOT_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16 + 2 * SOFTMAX_WARPS * 4;
+    static constexpr int BYTES = 1024 + SLOTS * SLOT_BYTES + 3 * PARTS * ROWS * 4 + BARS * 8 + 16 + 2 * SOFTMAX_WARPS * 4 + 16;
 };
 
 template <int P, bool CAP, bool BIAS>
@@ -328,8 +377,8 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    float* exchange = reinterpret_cast<float*>(gen + SLOTS * Shared::SLOT_BYTES);   // [2][PARTS][128]
-    const uint32_t bars = base + SLOTS * Shared::SLOT_BYTES + 2 * PARTS * ROWS * 4;
+    float* exchange = reinterpret_cast<float*>(gen + SLOTS * Shared::SLOT_BYTES);   // [3][PARTS][128]
+    const uint32_t bars = base + SLOTS * Shared::SLOT_BYTES + 3 * PARTS * ROWS * 4;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (SLOTS + s); };
     auto s_full = [&](int i) { return bars + 8u * (2 * SLOTS + i); };
@@ -339,6 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* doc_span = const_cast<int*>(reinterpret_cast<volatile int*>(tmem_slot + 2));   // [2]
     volatile int* agreed = reinterpret_cast<volatile int*>(tmem_slot + 4);              // [2][SOFTMAX_WARPS]: tile parity, warp
+    volatile int* by_row = agreed + 2 * SOFTMAX_WARPS;                                  // [4]: what each quadrant found
 
     const AttentionArgs& a = f.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -355,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         bar_init(o_full, 1);
         bar_init(o_empty, SOFTMAX_WARPS);
         bar_init(q_ready, SOFTMAX_WARPS);
-        *stop = 0;
+        *stop = by_row[0] = by_row[1] = by_row[2] = by_row[3] = 0;
         doc_span[0] = 0x7fffffff;
         doc_span[1] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -370,18 +420,19 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             atomicMax(&doc_span[1], d);
         }
     }
+    const int64_t image0 = (int64_t(b) * kv_heads + g) * k_tiles;
+    const int tiles_end = (max(sight.keys_end(min(q0 + ROWS, tq) - 1 + sight.shift), 0) + KT - 1) / KT;
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
     Walk walk;
     walk.begin = walk.halves = 0;
-    walk.end = (max(sight.keys_end(min(q0 + ROWS, tq) - 1 + sight.shift), 0) + KT - 1) / KT;
+    walk.end = tiles_end;
     walk.range = sight.docs ? f.doc_range + int64_t(b) * k_tiles : nullptr;
     walk.lo = sight.docs && doc_span[1] < 0 ? INFINITY : __int_as_float(doc_span[0]);
     walk.hi = doc_span[1] < 0 ? -1.f : __int_as_float(doc_span[1]);
     walk.share();
-    const int64_t image0 = (int64_t(b) * kv_heads + g) * k_tiles;
 
     if (warp == LOAD_WARP) {
         if (lane == 0) {
@@ -445,6 +496,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         {
             float x[SHARE];
             load_row_part<SHARE>(a.q.p + b * a.q.bs + int64_t(on ? q : 0) * a.q.ts + h * a.q.hs, part * SHARE, dim, on, f.q_vec, x);
+            if (units_by_row(f.k_scale + image0, f.v_scale + image0, tiles_end, 32 * part + lane, 32 * PARTS)) by_row[quad] = 1;
             exchange[part * ROWS + row] = largest(x);
             row_sync(quad);
             q_scale = tile_scale(row_max(exchange, row));
@@ -455,8 +507,10 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             if (lane == 0) bar_arrive(q_ready);
             row_sync(quad);
         }
+        auto arithmetic = [&](auto units) {
+        constexpr bool BY_ROWS = decltype(units)::value;
         const ScoreOf score(a, h);
-        const float cap2 = score.cap2, slope2 = score.slope2;
+        [[maybe_unused]] const float cap2 = score.cap2, slope2 = score.slope2;
         float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_before = 0.f;
 #pragma unroll
         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
@@ -481,7 +535,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
         for (int next; t >= 0; t = next, i++) {
             const int k0 = t * KT + KEYS * part;
-            const float mul = q_scale * k_next * score.mul, v_scale = v_next;
+            const float mul = BY_ROWS ? q_scale * score.mul : q_scale * k_next * score.mul;
+            float v_scale = v_next;
+            const int64_t row0 = (image0 + t) * ROWS + KEYS * part;
             const bool by_docs = docs_next;
             next = walk.from(t + 1);
             if (next >= 0) {   // a tile ahead: a load takes longer than the waits below should
@@ -498,6 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 uint32_t r[KEYS];
                 tmem_load(at, r);
                 tmem_wait_load();
+                if constexpr (BY_ROWS) times_rows(r, f.k_rows + row0);
 #pragma unroll
                 for (int c = 0; c < KEYS; c++) s[c] = __uint_as_float(r[c]) * mul;
             }
@@ -539,6 +596,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 s[c] = ex2(s[c] - from);
                 sums[c & 3] += s[c];
             }
+            if constexpr (BY_ROWS) {   // the largest weight times unit of a row sets the unit of its weights
+                times_rows(s, f.v_rows + row0, 0.5f);   // (in range whatever the values are)
+                float* units = exchange + 2 * PARTS * ROWS;
+                units[part * ROWS + row] = largest(s);
+                row_sync(quad);
+                const float own = tile_scale(row_max(units, row));
+                v_scale = own * 2.f;
+#pragma unroll
+                for (int c = 0; c < KEYS; c++) s[c] *= 1.f / own;
+            }
             store_halves<KEYS>(at, s, 1.f);
             tmem_wait_store();
             fence_before();
@@ -576,6 +643,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + log2f(l) : -INFINITY;
             }
         }
+        };
+        if (__builtin_expect(by_row[quad] == 0, 1)) arithmetic(std::false_type{});
+        else arithmetic(std::true_type{});
     }
     fence_before();
     __syncthreads();
@@ -617,13 +687,9 @@ __device__ __forceinline__ void fetch_half_image(uint32_t dst, const uint8_t* im
 // The largest of what a row's four threads hold, exchanged through shared memory: meeting `count` of the quadrant's warps.
 // (A barrier with a bounded wait: a warp that gave up does not come.  Two meetings in turn use different cells: a cell is
 // written again only after the meeting between, to which everybody came after reading it.)
-template <int N>
-__device__ __forceinline__ bool row_largest(const float (&x)[N], float* exchange, uint32_t meet, uint32_t count, int part, int row, volatile int* stop, int* status, float& most) {
+__device__ __forceinline__ bool row_largest(float& most, float* exchange, uint32_t meet, uint32_t count, int part, int row, volatile int* stop, int* status) {
     float* cell = exchange + (count & 1) * PARTS * ROWS;
-    float top = 0.f;   // (an infinity may set the unit: it reaches every element of the row's sum anyway)
-#pragma unroll
-    for (int c = 0; c < N; c++) top = fmaxf(top, fabsf(x[c]));
-    cell[part * ROWS + row] = top;
+    cell[part * ROWS + row] = most;
     __syncwarp();
     if ((threadIdx.x & 31) == 0) bar_arrive(meet);
     if (!bar_wait_warp(meet, count & 1, stop, status, GAVE_UP_MEET)) return false;
@@ -639,7 +705,7 @@ struct QueryGradShared {
     static constexpr int SLOTS = 3;   // of keys and of values
     static constexpr int SLOT_BYTES = 2 * P * SUB_BYTES;
     static constexpr int BARS = 4 * SLOTS + 11;
-    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16;
+    static constexpr int BYTES = 1024 + 2 * SLOTS * SLOT_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 32;
 };
 
 template <int P, bool CAP, bool BIAS>
@@ -662,6 +728,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                    ds_ready = own_ready + 32, acc_full = own_ready + 40, acc_taken = own_ready + 48, meet = own_ready + 56;   // meet: one for each quadrant
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (bars - base) + Shared::BARS * 8);
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* by_row = stop + 1;   // [4]: what each quadrant found
 
     const AttentionArgs& a = f.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -683,7 +750,10 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         bar_init(ds_ready, SOFTMAX_WARPS);
         bar_init(acc_full, 1);
         bar_init(acc_taken, SOFTMAX_WARPS);
-        for (int i = 0; i < 4; i++) bar_init(meet + 8 * i, PARTS);
+        for (int i = 0; i < 4; i++) {
+            bar_init(meet + 8 * i, PARTS);
+            by_row[i] = 0;
+        }
         *stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -775,6 +845,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             const Strided4& src = which ? a.dout : a.q;
             float x[SHARE];
             load_row_part<SHARE>(src.p + b * src.bs + int64_t(on ? q : 0) * src.ts + h * src.hs, part * SHARE, dim, on, which ? f.dout.vec : f.q.vec, x);
+            if (!which && units_by_row(f.k.scale + image0, f.v.scale + image0, (keys_end + ROWS - 1) / ROWS, 32 * part + lane, 32 * PARTS)) by_row[quad] = 1;
             exchange[part * ROWS + row] = largest(x);
             row_sync(quad);
             own_scale[which] = tile_scale(row_max(exchange, row));
@@ -786,6 +857,8 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(own_ready);
+        auto arithmetic = [&](auto units) {
+        constexpr bool BY_ROWS = decltype(units)::value;
         const ScoreOf score(a, h);
         float acc[SHARE], factor = 0.f;   // of the accumulator that has not been emptied yet
 #pragma unroll
@@ -811,15 +884,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         float k_next = t >= 0 ? __ldg(f.k.scale + image0 + (t >> 1)) : 0.f, v_next = t >= 0 ? __ldg(f.v.scale + image0 + (t >> 1)) : 0.f;
         for (int next; t >= 0; t = next, n++) {
             const int k0 = t * GT + KEYS * part;
-            const float k_scale = k_next, v_scale = v_next;
             const bool by_docs = docs_next;
+            const float k_scale = BY_ROWS ? 1.f / ROW_TOP : k_next;
+            const float mul = BY_ROWS ? own_scale[0] * score.mul : own_scale[0] * k_next * score.mul, dp_mul = BY_ROWS ? own_scale[1] : own_scale[1] * v_next;
+            const int64_t row0 = image0 * ROWS + t * GT + KEYS * part;
             next = walk.from(t + 1);
             if (next >= 0) {   // a tile ahead
                 docs_next = !walk.one_document(next);
                 k_next = __ldg(f.k.scale + image0 + (next >> 1));
                 v_next = __ldg(f.v.scale + image0 + (next >> 1));
             }
-            const float mul = own_scale[0] * k_scale * score.mul, dp_mul = own_scale[1] * v_scale;
             float p[KEYS];   // weights, times the scores' bend
             uint32_t r[KEYS];
             if (!bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
@@ -829,6 +903,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(s_taken);
+            if constexpr (BY_ROWS) times_rows(r, f.k.rows + row0);
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
                 float s = __uint_as_float(r[c]) * mul, bend = 1.f;
@@ -852,12 +927,16 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             fence_after();
             tmem_load(lanes + C_DP + KEYS * part, r);
             tmem_wait_load();
+            if constexpr (BY_ROWS) times_rows(r, f.v.rows + row0);
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
                 p[c] = p[c] == 0.f ? 0.f : p[c] * fmaf(__uint_as_float(r[c]), dp_mul, -delta);
             }
-            float most;
-            if (!row_largest(p, exchange, meet + 8 * quad, n, part, row, stop, f.status, most)) { ok = false; break; }
+            if constexpr (BY_ROWS) times_rows(p, f.k.rows + row0, ROW_TOP);
+            float most = 0.f;   // (an infinity may set the unit: it reaches every element of the row's sum anyway)
+#pragma unroll
+            for (int c = 0; c < KEYS; c++) most = fmaxf(most, fabsf(p[c]));
+            if (!row_largest(most, exchange, meet + 8 * quad, n, part, row, stop, f.status)) { ok = false; break; }
             const float unit = tile_scale(most);
             factor = unit * k_scale * a.scale;
             store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f / unit);
@@ -873,6 +952,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
                 for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
             store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, 1.f);
         }
+        };
+        if (__builtin_expect(by_row[quad] == 0, 1)) arithmetic(std::false_type{});
+        else arithmetic(std::true_type{});
     }
     fence_before();
     __syncthreads();
@@ -889,7 +971,7 @@ template <int P>
 struct KeyGradShared {
     static constexpr int SLOTS = P == 2 ? 2 : 4;   // of queries and of the outputs' gradients
     static constexpr int DATA_BYTES = 2 * P * SUB_BYTES;
-    static constexpr int STATS_BYTES = 2 * GT * 4;
+    static constexpr int STATS_BYTES = 4 * GT * 4;   // of the tile's queries: logarithms, deltas, units of q and of do
     static constexpr int OWN_BYTES = P == 2 ? image_bytes(P) : 0;
     static constexpr int BARS = 4 * SLOTS + 14;
     static constexpr int BYTES = 1024 + OWN_BYTES + 2 * SLOTS * DATA_BYTES + SLOTS * STATS_BYTES + 2 * PARTS * ROWS * 4 + BARS * 8 + 16;
@@ -922,7 +1004,10 @@ struct HeadWalk {
 constexpr int KEY_THREADS = 32 * (SOFTMAX_WARPS + 4), KEY_REGS = 96, KEY_REGS_MANY = 112, KEY_REGS_FEW = 32;
 static_assert(32 * SOFTMAX_WARPS * KEY_REGS_MANY + 128 * KEY_REGS_FEW <= KEY_THREADS * KEY_REGS, "the split must fit what the block was launched with");
 
-template <int P, bool CAP, bool BIAS>
+// Two kernels: the second takes the blocks whose queries have units by row (a block of the other kernel returns at once).
+// In one kernel the two loops took registers from one another: 1083 us instead of 980 for the usual one (2 x 4096 tokens, 16
+// heads of 128); blocks that return take 15 of them (4 with one block an SM).
+template <int P, bool CAP, bool BIAS, bool BY_ROWS>
 __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const GradArgs f) {
     using Shared = KeyGradShared<P>;
     constexpr int SLOTS = Shared::SLOTS, DATA = Shared::DATA_BYTES, STATS = Shared::STATS_BYTES, DP = 64 * P, SHARE = DP / PARTS, QUERIES = GT / PARTS;
@@ -974,6 +1059,8 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         *stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    const bool by_rows = units_by_row(f.q.scale + head0 * q_tiles, f.dout.scale + head0 * q_tiles, group * q_tiles, int(threadIdx.x), KEY_THREADS);
+    if (bool(__syncthreads_or(by_rows)) != BY_ROWS) return;
     if (warp == MMA_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), 512);
     fence_before();
     __syncthreads();
@@ -1008,10 +1095,14 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                     const int64_t image0 = (head0 + at.head) * q_tiles, row0 = (head0 + at.head) * q_tiles * ROWS + int64_t(at.t) * GT;
                     ok = bar_wait(q_empty(n), phase, stop, f.status, GAVE_UP_SLOT);
                     if (!ok) break;
-                    bar_expect(q_full(n), DATA + STATS);
+                    bar_expect(q_full(n), DATA + (BY_ROWS ? 4 : 2) * GT * 4);
                     fetch_half_image<P>(q_slot(n), f.q.image, image0, at.t, q_full(n));
                     bulk_load(base + stats(n), f.q.lse + row0, GT * 4, q_full(n));
                     bulk_load(base + stats(n) + GT * 4, f.dout.delta + row0, GT * 4, q_full(n));
+                    if constexpr (BY_ROWS) {
+                        bulk_load(base + stats(n) + 2 * GT * 4, f.q.rows + row0, GT * 4, q_full(n));
+                        bulk_load(base + stats(n) + 3 * GT * 4, f.dout.rows + row0, GT * 4, q_full(n));
+                    }
                     ok = bar_wait(o_empty(n), phase, stop, f.status, GAVE_UP_SLOT);
                     if (!ok) { n++; break; }
                     bar_expect(o_full(n), DATA);
@@ -1070,7 +1161,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
         const bool on = j < tk && sight.key_used(j);
         const float doc = on && sight.docs ? sight.docs[j] : 0.f;
-        const float k_scale = __ldg(f.k.scale + own_image), v_scale = __ldg(f.v.scale + own_image);
+        const float k_scale = __ldg(f.k.rows + own_image * ROWS + row), v_scale = __ldg(f.v.rows + own_image * ROWS + row);
 #pragma unroll
         for (int which = 0; which < (P == 1 ? 2 : 1); which++) {   // the block's own operands, in their images' units
             const Strided4& src = which ? a.v : a.k;
@@ -1108,9 +1199,11 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         float q_next = 0.f, o_next = 0.f, slope_next = 0.f;
         bool docs_next = false;
         auto look = [&]() {   // what belongs to the tile of queries that `at` stands on
-            const int64_t image = (head0 + at.head) * q_tiles + (at.t >> 1);
-            q_next = __ldg(f.q.scale + image);
-            o_next = __ldg(f.dout.scale + image);
+            if constexpr (!BY_ROWS) {
+                const int64_t image = (head0 + at.head) * q_tiles + (at.t >> 1);
+                q_next = __ldg(f.q.scale + image);
+                o_next = __ldg(f.dout.scale + image);
+            }
             docs_next = !walk.one_document(at.t);
             if constexpr (BIAS) slope_next = __ldg(a.slopes + g * group + at.head) * LOG2E;
         };
@@ -1118,30 +1211,33 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         const ScoreOf score(a, g * group);   // (but for the slope the same for every head)
         for (bool more = any; more; n++) {
             const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
-            const float q_scale = q_next, o_scale = o_next, slope2 = slope_next;
             const bool by_docs = docs_next;
+            [[maybe_unused]] const float slope2 = slope_next;
+            const float q_scale = BY_ROWS ? 1.f / ROW_TOP : q_next, o_scale = BY_ROWS ? 1.f / ROW_TOP : o_next;
+            const float mul = BY_ROWS ? k_scale * score.mul : q_next * k_scale * score.mul, dp_mul = BY_ROWS ? v_scale : o_next * v_scale;
             more = at.next();
             if (more) look();   // a tile ahead
-            const float mul = q_scale * k_scale * score.mul, dp_mul = o_scale * v_scale;
             if (!ok || !bar_wait_warp(q_full(n), (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA) || !bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
             fence_after();
             const float4* lse = reinterpret_cast<const float4*>(gen + stats(n)) + QUERIES / 4 * part;
             const float4* delta = lse + GT / 4;
+            [[maybe_unused]] const float4 *q_unit = lse + 2 * GT / 4, *o_unit = lse + 3 * GT / 4;
             const bool partly = by_docs || (sight.causal && q0 + sight.shift < k0 + ROWS - 1 && k0 + ROWS - 1 >= sight.prefix);
             const int behind = sight.causal && j >= sight.prefix ? j - sight.shift - q0 : 0;   // queries in front of the key
             static_assert(QUERIES == 16, "a thread's columns of a tile");
-            float p[QUERIES], bends[CAP ? QUERIES : 1], most;   // weights, and the scores' bend
+            float p[QUERIES], most = 0.f;   // weights
+            [[maybe_unused]] float bends[CAP ? QUERIES : 1];
             uint32_t r[QUERIES];
             {
                 tmem_load(lanes + C_S + QUERIES * part, r);
                 tmem_wait_load();
 #pragma unroll
                 for (int c = 0; c < QUERIES; c += 4) {
-                    const float4 ls = lse[c / 4];
-                    const float l4[4] = {ls.x, ls.y, ls.z, ls.w};
+                    const float4 ls = lse[c / 4], one = make_float4(1.f, 1.f, 1.f, 1.f), qu = BY_ROWS ? q_unit[c / 4] : one, ou = BY_ROWS ? o_unit[c / 4] : one;
+                    const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, q4[4] = {qu.x, qu.y, qu.z, qu.w}, o4[4] = {ou.x, ou.y, ou.z, ou.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float s = __uint_as_float(r[c + e]) * mul;
+                        float s = (BY_ROWS ? __uint_as_float(r[c + e]) * q4[e] : __uint_as_float(r[c + e])) * mul;
                         if constexpr (CAP) {
                             const float w = tanh_exact(s);
                             bends[c + e] = fmaf(-w, w, 1.f);
@@ -1154,12 +1250,24 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                             if (c + e < behind || (by_docs && (q >= tq || q + sight.shift < 0 || __ldg(sight.docs + q + sight.shift) != doc))) w = 0.f;
                         }
                         p[c + e] = w;
+                        most = fmaxf(most, BY_ROWS ? w * (o4[e] * ROW_TOP) : w);
                     }
                 }
-                if (!row_largest(p, exchange, meet + 8 * quad, 2 * n, part, row, stop, f.status, most)) { ok = false; break; }
+                if (!row_largest(most, exchange, meet + 8 * quad, 2 * n, part, row, stop, f.status)) { ok = false; break; }
                 const float unit = tile_scale(most);
                 dv_factor = unit * o_scale;
-                store_halves<QUERIES>(lanes + C_S + QUERIES * part, p, 1.f / unit);
+                if constexpr (BY_ROWS) {
+                    float x[QUERIES];
+#pragma unroll
+                    for (int c = 0; c < QUERIES; c += 4) {
+                        const float4 ou = o_unit[c / 4];
+                        const float o4[4] = {ou.x, ou.y, ou.z, ou.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[c + e] = p[c + e] * (o4[e] * ROW_TOP);
+                    }
+                    store_halves<QUERIES>(lanes + C_S + QUERIES * part, x, 1.f / unit);
+                } else
+                    store_halves<QUERIES>(lanes + C_S + QUERIES * part, p, 1.f / unit);
             }
             if constexpr (CAP)
 #pragma unroll
@@ -1173,16 +1281,20 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             fence_after();
             tmem_load(lanes + C_DP + QUERIES * part, r);
             tmem_wait_load();
+            most = 0.f;
 #pragma unroll
             for (int c = 0; c < QUERIES; c += 4) {
-                const float4 de = delta[c / 4];
-                const float d4[4] = {de.x, de.y, de.z, de.w};
+                const float4 de = delta[c / 4], one = make_float4(1.f, 1.f, 1.f, 1.f), qu = BY_ROWS ? q_unit[c / 4] : one, ou = BY_ROWS ? o_unit[c / 4] : one;
+                const float d4[4] = {de.x, de.y, de.z, de.w}, q4[4] = {qu.x, qu.y, qu.z, qu.w}, o4[4] = {ou.x, ou.y, ou.z, ou.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]);
+                    const float x = BY_ROWS ? __uint_as_float(r[c + e]) * o4[e] : __uint_as_float(r[c + e]);
+                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * fmaf(x, dp_mul, -d4[e]);
+                    if constexpr (BY_ROWS) p[c + e] *= q4[e] * ROW_TOP;
+                    most = fmaxf(most, fabsf(p[c + e]));
                 }
             }
-            if (!row_largest(p, exchange, meet + 8 * quad, 2 * n + 1, part, row, stop, f.status, most)) { ok = false; break; }
+            if (!row_largest(most, exchange, meet + 8 * quad, 2 * n + 1, part, row, stop, f.status)) { ok = false; break; }
             const float unit = tile_scale(most);
             dk_factor = unit * q_scale * a.scale;
             store_halves<QUERIES>(lanes + C_DP + QUERIES * part, p, 1.f / unit);
@@ -1262,6 +1374,7 @@ ImageJob image_job(Cut& cut, const Strided4& src, const AttentionShape& s, bool 
     const int64_t n = s.batch * j.heads * j.tiles;
     j.image = cut.take<uint8_t>(n * image_bytes(P));
     j.scale = cut.take<float>(n);
+    j.rows = cut.take<float>(n * ROWS);
     return j;
 }
 cudaError_t images(const ImageArgs& im, int jobs, int P, CUstream_st* stream) {
@@ -1281,11 +1394,15 @@ cudaError_t grad_kernel(const GradArgs& f, dim3 grid, CUstream_st* stream) {
         constexpr bool CAP = decltype(c)::value, BIAS = decltype(s)::value;
         if constexpr (KEYS) {
             // its warps share out the registers it is launched with: fewer than that sum would leave them waiting
-            cudaFuncAttributes attr;
-            cudaError_t e = cudaFuncGetAttributes(&attr, (const void*)adb_attention_tc_dkv<P, CAP, BIAS>);
-            if (e != cudaSuccess) return e;
-            if (attr.numRegs < KEY_REGS) return cudaErrorInvalidKernelImage;
-            return launch(adb_attention_tc_dkv<P, CAP, BIAS>, grid, KEY_THREADS, KeyGradShared<P>::BYTES, stream, f);
+            auto one = [&](auto kernel) {
+                cudaFuncAttributes attr;
+                cudaError_t e = cudaFuncGetAttributes(&attr, (const void*)kernel);
+                if (e != cudaSuccess) return e;
+                if (attr.numRegs < KEY_REGS) return cudaErrorInvalidKernelImage;
+                return launch(kernel, grid, KEY_THREADS, KeyGradShared<P>::BYTES, stream, f);
+            };
+            const cudaError_t e = one(adb_attention_tc_dkv<P, CAP, BIAS, false>);
+            return e == cudaSuccess ? one(adb_attention_tc_dkv<P, CAP, BIAS, true>) : e;
         }
         else return launch(adb_attention_tc_dq<P, CAP, BIAS>, grid, THREADS, QueryGradShared<P>::BYTES, stream, f);
     };
@@ -1311,6 +1428,7 @@ int attention_tc_launch(const AttentionArgs& a, CUstream_st* stream, std::string
         f.a = a;
         f.k = im.job[0].image; f.v = im.job[1].image;
         f.k_scale = im.job[0].scale; f.v_scale = im.job[1].scale;
+        f.k_rows = im.job[0].rows; f.v_rows = im.job[1].rows;
         f.doc_range = im.job[0].docs;
         f.status = a.status;
         f.q_vec = fits16(a.q, s.dim);

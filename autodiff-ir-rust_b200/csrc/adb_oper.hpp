@@ -112,9 +112,9 @@ inline int64_t attention_ranges(const AttentionShape& s, int sm_count) {
 }
 inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
     if (!attention_uses_tc(s)) return s.batch * s.tq * s.heads * attention_ranges(s, sm_count) * (s.dim + 2);
-    // images of keys and values, a scale for each, document numbers; each part begins on a 256-byte boundary
+    // images of keys and values, their scales by tile and by row, document numbers; each part begins on a 256-byte boundary
     const int64_t tiles = attention_tc_tiles(s.tk), n = s.batch * s.kv_heads * tiles, shares = attention_forward_shares(s, sm_count);
-    return 2 * (n * attention_panels(s.dim) * 8192 + n + 64) + 4 * s.batch * tiles + 64 +
+    return 2 * (n * (attention_panels(s.dim) * 8192 + 1 + ATTENTION_TC_TILE) + 128) + 4 * s.batch * tiles + 64 +
            (shares > 1 ? s.batch * s.tq * s.heads * shares * (s.dim + 2) : 0);
 }
 // The gradient takes them whatever the count of queries: the CUDA-core kernels' tiles of 64 are just as empty.
@@ -127,7 +127,7 @@ inline int64_t attention_grad_workspace(const AttentionShape& s, int sm_count) {
     const int64_t nk = s.batch * s.kv_heads * kt, nq = s.batch * s.heads * qt;
     const int64_t q_shares = attention_dq_shares(s, sm_count), k_shares = attention_dkv_shares(s, sm_count);
     // images of four operands with their scales, logarithms and deltas in whole tiles, document numbers
-    return 2 * ((nk + nq) * attention_panels(s.dim) * 8192 + nk + nq + 128) + 2 * (nq * ATTENTION_TC_TILE + 64) +
+    return 2 * ((nk + nq) * (attention_panels(s.dim) * 8192 + 1 + ATTENTION_TC_TILE) + 256) + 2 * (nq * ATTENTION_TC_TILE + 64) +
            4 * s.batch * (kt + qt) + 128 + (q_shares > 1 ? q_shares * s.batch * s.tq * s.heads * s.dim + 64 : 0) +
            (k_shares > 1 ? 2 * (k_shares * s.batch * s.tk * s.kv_heads * s.dim + 64) : 0);
 }

@@ -1,8 +1,9 @@
 // fp32 products on the fp16 tensor cores of sm_100a: operands as sums of two halves, and the tcgen05 instructions for them.
 //
-// An fp32 value x is held as s (hi + lo) with s a power of two shared by a tile and hi, lo fp16: hi is x / s rounded to
-// 11 bits, lo the rest rounded to 11 more.  s puts the tile's largest magnitude into [2^14, 2^15), so that a value 2^-17
-// of it still has all 22 bits and the error of any value is below 2^-39 of the largest.  A product is
+// An fp32 value x is held as s (hi + lo) with s a power of two and hi, lo fp16: hi is x / s rounded to 11 bits, lo the rest
+// rounded to 11 more.  s is a row's own, or shared by the rows of a tile when they are of similar size: it puts the largest
+// magnitude into [2^14, 2^15), so that a value 2^-17 of it still has all 22 bits and the error of any value is below 2^-39
+// of the largest.  A product is
 // lo.hi + hi.lo + hi.hi in fp32 accumulators (lo.lo is below 2^-22 of it): three fp16 instructions at twice the rate of the
 // tf32 ones that the dot kernels use, and half their bytes in shared memory.
 //

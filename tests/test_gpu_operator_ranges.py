@@ -85,3 +85,36 @@ def test_keys_of_little_weight(no_floors, d, few):
         for n, x in oc.attention_run(dev, c).items():
             oc.close(n, x, *ref[n])
         dev.close()
+
+
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("ratio", [2.0 ** -9, 2.0 ** -12, 2.0 ** -20])
+def test_documents_token_by_token_in_one_tile(no_floors, d, ratio):
+    c = _side_by_side(d, ratio)
+    _tc_and_fp32(c)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(cap=4.0)])
+@pytest.mark.parametrize("tq,tk,heads,d", [(700, 700, 2, 128), (130, 4000, 1, 64), (300, 300, 2, 96)])
+def test_rows_of_every_size(no_floors, kw, tq, tk, heads, d):
+    """values and output gradients whose rows differ by up to 2^60, in every mixture; the middle case shares a tile's walk
+    between blocks.  A row's results are made of what it sees, the largest first."""
+    c = oc.attention_case(1, tq, tk, heads, heads, d, seed=tq, **kw)
+    rng = np.random.default_rng(11)
+    for n in ("v", "do"):
+        size = rng.uniform(-30, 30, c[n].shape[1])
+        size[:200] = rng.uniform(-8, 0, 200)[:len(size[:200])]     # a tile of similar rows, one across the border, the rest mixed
+        c[n] *= np.exp2(np.round(size)).astype(np.float32)[None, :, None, None]
+    c["k"][:, ::7] *= np.float32(2.0 ** -14)
+    c["q"][:, ::5] *= np.float32(2.0 ** -14)
+    _tc_and_fp32(c)
+
+
+def test_rows_of_zeros_beside_others(no_floors):
+    """rows of zeros neither set a tile's unit nor need one"""
+    c = oc.attention_case(1, 260, 260, 2, 1, 64, seed=8)
+    for n in ("q", "k", "v", "do"):
+        c[n][:, 3::4] = 0
+    _tc_and_fp32(c)
+    c["do"][:], c["v"][:] = 0, 0
+    _tc_and_fp32(c)
