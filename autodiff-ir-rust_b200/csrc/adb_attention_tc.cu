@@ -261,15 +261,26 @@ __device__ __forceinline__ bool units_by_row(const float* one, const float* othe
     for (int i = thread; i < n; i += threads) any |= fminf(__ldg(one + i), __ldg(other + i)) < 0.f;   // (both loads at once)
     return any;
 }
-// a tile's columns times the units of the rows they stand for (16-byte boundary)
+// What a row's unit is multiplied with to give its largest magnitude, within a factor of two.
+constexpr float ROW_TOP = 16384.f;
+// A product of units that may lie at opposite ends of the range: x * a row's factor * a column's, the factor below one first.
+// Only a product that is out of range itself, or whose factors are 2^186 apart, leaves it.
+struct RowFactor {
+    float before, after;
+    __device__ __forceinline__ explicit RowFactor(float f) : before(fabsf(f) < 1.f ? f * (1.f / ROW_TOP) : 1.f / ROW_TOP), after(fabsf(f) < 1.f ? ROW_TOP : f * ROW_TOP) {}
+    __device__ __forceinline__ float operator()(float x, float column) const { return x * before * column * after; }
+};
+// one factor for a tile: finite, so that zeros stay zeros
+__device__ __forceinline__ float in_range(float f) { return fmaxf(fminf(f, 3.4e38f), -3.4e38f); }
+// a tile's columns times the units of the rows they stand for (16-byte boundary) and the row's own factor
 template <int N>
-__device__ __forceinline__ void times_rows(uint32_t (&r)[N], const float* units) {
+__device__ __forceinline__ void times_rows(uint32_t (&r)[N], const float* units, const RowFactor& own) {
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
         const float4 u = __ldg(reinterpret_cast<const float4*>(units + c));
         const float f[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int e = 0; e < 4; e++) r[c + e] = __float_as_uint(__uint_as_float(r[c + e]) * f[e]);
+        for (int e = 0; e < 4; e++) r[c + e] = __float_as_uint(own(__uint_as_float(r[c + e]), f[e]));
     }
 }
 template <int N>
@@ -282,8 +293,6 @@ __device__ __forceinline__ void times_rows(float (&x)[N], const float* units, fl
         for (int e = 0; e < 4; e++) x[c + e] *= f[e] * factor;
     }
 }
-// What a row's unit is multiplied with to give its largest magnitude, within a factor of two.
-constexpr float ROW_TOP = 16384.f;
 // the warps that share a quadrant's rows
 __device__ __forceinline__ void row_sync(int quad) { asm volatile("bar.sync %0, %1;" ::"r"(1 + quad), "n"(32 * PARTS) : "memory"); }
 // largest, or sum, of what the row's threads put down
@@ -535,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
         for (int next; t >= 0; t = next, i++) {
             const int k0 = t * KT + KEYS * part;
-            const float mul = BY_ROWS ? q_scale * score.mul : q_scale * k_next * score.mul;
+            const float mul = BY_ROWS ? 1.f : in_range(q_scale * k_next * score.mul);
             float v_scale = v_next;
             const int64_t row0 = (image0 + t) * ROWS + KEYS * part;
             const bool by_docs = docs_next;
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
                 uint32_t r[KEYS];
                 tmem_load(at, r);
                 tmem_wait_load();
-                if constexpr (BY_ROWS) times_rows(r, f.k_rows + row0);
+                if constexpr (BY_ROWS) times_rows(r, f.k_rows + row0, RowFactor(q_scale * score.mul));
 #pragma unroll
                 for (int c = 0; c < KEYS; c++) s[c] = __uint_as_float(r[c]) * mul;
             }
@@ -585,8 +594,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
 #pragma unroll
             for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
             if (!ok) break;
-            // weights in units of the tile's own largest, sums and results in units of the largest so far
-            const float tile_top = row_max(cell, row), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
+            // Weights in units of the tile's own largest, sums and results in units of the largest so far, both rounded up
+            // to powers of two: what is rescaled keeps its bits, and a unit of values near 2^-126 is exact among the subnormals.
+            const float tile_top = ceilf(row_max(cell, row)), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
             const float from = (tile_top == -INFINITY ? 0.f : tile_top) - P_SHIFT;
             const float fade = ex2(m - base), unit = ex2(tile_top - base - P_SHIFT);
             m = top;
@@ -886,7 +896,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             const int k0 = t * GT + KEYS * part;
             const bool by_docs = docs_next;
             const float k_scale = BY_ROWS ? 1.f / ROW_TOP : k_next;
-            const float mul = BY_ROWS ? own_scale[0] * score.mul : own_scale[0] * k_next * score.mul, dp_mul = BY_ROWS ? own_scale[1] : own_scale[1] * v_next;
+            const float mul = BY_ROWS ? 1.f : in_range(own_scale[0] * k_next * score.mul), dp_mul = BY_ROWS ? 1.f : in_range(own_scale[1] * v_next);
             const int64_t row0 = image0 * ROWS + t * GT + KEYS * part;
             next = walk.from(t + 1);
             if (next >= 0) {   // a tile ahead
@@ -903,7 +913,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(s_taken);
-            if constexpr (BY_ROWS) times_rows(r, f.k.rows + row0);
+            if constexpr (BY_ROWS) times_rows(r, f.k.rows + row0, RowFactor(own_scale[0] * score.mul));
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
                 float s = __uint_as_float(r[c]) * mul, bend = 1.f;
@@ -927,7 +937,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             fence_after();
             tmem_load(lanes + C_DP + KEYS * part, r);
             tmem_wait_load();
-            if constexpr (BY_ROWS) times_rows(r, f.v.rows + row0);
+            if constexpr (BY_ROWS) times_rows(r, f.v.rows + row0, RowFactor(own_scale[1]));
 #pragma unroll
             for (int c = 0; c < KEYS; c++) {
                 p[c] = p[c] == 0.f ? 0.f : p[c] * fmaf(__uint_as_float(r[c]), dp_mul, -delta);
@@ -938,7 +948,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             for (int c = 0; c < KEYS; c++) most = fmaxf(most, fabsf(p[c]));
             if (!row_largest(most, exchange, meet + 8 * quad, n, part, row, stop, f.status)) { ok = false; break; }
             const float unit = tile_scale(most);
-            factor = unit * k_scale * a.scale;
+            factor = unit * k_scale;   // (powers of two: exact down to 2^-149)
             store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f / unit);
             tmem_wait_store();
             fence_before();
@@ -950,7 +960,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
             if (!on)
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, 1.f);
+            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, a.scale);
         }
         };
         if (__builtin_expect(by_row[quad] == 0, 1)) arithmetic(std::false_type{});
@@ -1209,12 +1219,13 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
         };
         if (any) look();
         const ScoreOf score(a, g * group);   // (but for the slope the same for every head)
+        [[maybe_unused]] const RowFactor own_q(k_scale * score.mul), own_o(v_scale);
         for (bool more = any; more; n++) {
             const int q0 = at.t * GT + QUERIES * part;   // the thread's first query
             const bool by_docs = docs_next;
             [[maybe_unused]] const float slope2 = slope_next;
             const float q_scale = BY_ROWS ? 1.f / ROW_TOP : q_next, o_scale = BY_ROWS ? 1.f / ROW_TOP : o_next;
-            const float mul = BY_ROWS ? k_scale * score.mul : q_next * k_scale * score.mul, dp_mul = BY_ROWS ? v_scale : o_next * v_scale;
+            const float mul = BY_ROWS ? 1.f : in_range(q_next * k_scale * score.mul), dp_mul = BY_ROWS ? 1.f : in_range(o_next * v_scale);
             more = at.next();
             if (more) look();   // a tile ahead
             if (!ok || !bar_wait_warp(q_full(n), (n / SLOTS) & 1, stop, f.status, GAVE_UP_DATA) || !bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
@@ -1237,7 +1248,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                     const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, q4[4] = {qu.x, qu.y, qu.z, qu.w}, o4[4] = {ou.x, ou.y, ou.z, ou.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float s = (BY_ROWS ? __uint_as_float(r[c + e]) * q4[e] : __uint_as_float(r[c + e])) * mul;
+                        float s = BY_ROWS ? own_q(__uint_as_float(r[c + e]), q4[e]) : __uint_as_float(r[c + e]) * mul;
                         if constexpr (CAP) {
                             const float w = tanh_exact(s);
                             bends[c + e] = fmaf(-w, w, 1.f);
@@ -1288,15 +1299,15 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
                 const float d4[4] = {de.x, de.y, de.z, de.w}, q4[4] = {qu.x, qu.y, qu.z, qu.w}, o4[4] = {ou.x, ou.y, ou.z, ou.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float x = BY_ROWS ? __uint_as_float(r[c + e]) * o4[e] : __uint_as_float(r[c + e]);
-                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * fmaf(x, dp_mul, -d4[e]);
+                    const float w = BY_ROWS ? own_o(__uint_as_float(r[c + e]), o4[e]) - d4[e] : fmaf(__uint_as_float(r[c + e]), dp_mul, -d4[e]);
+                    p[c + e] = p[c + e] == 0.f ? 0.f : p[c + e] * w;
                     if constexpr (BY_ROWS) p[c + e] *= q4[e] * ROW_TOP;
                     most = fmaxf(most, fabsf(p[c + e]));
                 }
             }
             if (!row_largest(most, exchange, meet + 8 * quad, 2 * n + 1, part, row, stop, f.status)) { ok = false; break; }
             const float unit = tile_scale(most);
-            dk_factor = unit * q_scale * a.scale;
+            dk_factor = unit * q_scale;   // (powers of two: exact down to 2^-149)
             store_halves<QUERIES>(lanes + C_DP + QUERIES * part, p, 1.f / unit);
             tmem_wait_store();
             fence_before();
@@ -1309,7 +1320,7 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
             if (!on)   // no query sees the key, whatever its row was compared with
 #pragma unroll
                 for (int c = 0; c < SHARE; c++) dk[c] = dv[c] = 0.f;
-            if (f.dk) store_row_part<SHARE>(f.dk + out_row, part * SHARE, dim, f.out_vec, dk, 1.f);
+            if (f.dk) store_row_part<SHARE>(f.dk + out_row, part * SHARE, dim, f.out_vec, dk, a.scale);
             if (f.dv) store_row_part<SHARE>(f.dv + out_row, part * SHARE, dim, f.out_vec, dv, 1.f);
         }
     }

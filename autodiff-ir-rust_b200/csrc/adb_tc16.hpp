@@ -173,10 +173,11 @@ __device__ __forceinline__ void tmem_store_halves(uint32_t taddr, const float* x
     for (int k = 0; k < 8; k++) halves(x[2 * k] * f, x[2 * k + 1] * f, r[k], r[8 + k]);
     tmem_store16(taddr, r);
 }
-// The power of two that divides a magnitude into [2^14, 2^15).  Exponents are kept within +-100, so that the factor and its
-// inverse are normal numbers; zero gets the smallest, so that a tile of zeros does not set the unit of a sum over tiles.
+// The power of two that divides a magnitude into [2^14, 2^15), whatever finite number it is: 2^113 for the largest.  It and
+// its inverse are normal numbers: from 2^-112 downwards it is 2^-126, of which half of fp16's smallest step is still less
+// than an fp32 subnormal.  Zero gets that too.
 __device__ __forceinline__ float tile_scale(float largest) {
-    const int e = min(max(int(__float_as_uint(fmaxf(largest, 0.f)) >> 23) - 127 - 14, -100), 100);
+    const int e = min(max(int(__float_as_uint(fmaxf(largest, 0.f)) >> 23) - 127 - 14, -126), 113);
     return __uint_as_float(uint32_t(e + 127) << 23);
 }
 __device__ __forceinline__ float finite_magnitude(float x) {

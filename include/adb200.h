@@ -66,7 +66,8 @@ typedef enum adb_status {
  *   allowed below in brackets), u8 n_results, n_results x u32 (distinct ids), u8 n_ints, n_ints x i64, u8 n_reals,
  *   n_reals x f32.  The counts are fixed.  A result that nothing needs is not computed where that saves work.
  *     30 RmsNorm       x scale [residual] -> y h; reals: eps
- *                      h = x + residual, y = h / sqrt(mean(h^2) + eps) * scale over the last axis
+ *                      h = x + residual, y = h / sqrt(mean(h^2) + eps) * scale over the last axis; squares are summed in
+ *                      fp32 (a row whose squares overflow gives zeros)
  *     31 RmsNormGrad   h scale dy [dh] -> dx dscale; reals: eps       (dx is the residual's gradient too)
  *     32 Rotary        x[B,T,H,D] table[2,P] [positions [T] or [B,T]] -> y; ints: interleaved, inverse, offset;
  *                      reals: gain.  The first 2 P elements of every head, taken in pairs (2i, 2i+1) or (i, P+i), are
@@ -81,6 +82,9 @@ typedef enum adb_status {
  *                      causal: j <= p or j < prefix; documents: the numbers at p and j agree and are not negative.
  *                      Causal or with lengths, a query with p < 0 sees nothing.  A query that sees nothing: out 0, lse -inf.
  *                      Lengths and prefixes are cut to [0, Tk] and to whole numbers (NaN: 0).
+ *                      Results are finite for finite operands as long as sums of |v| over the keys stay within fp32's range.
+ *                      Rows behind a sequence's length and rows of padding are not read; an infinity or a NaN in any
+ *                      other row may reach every query of its sequence and head.
  *     34 AttentionGrad q k v [slopes] [documents] [prefix] [lengths] out lse dout -> dq dk dv; ints, reals as 33.
  *                      No gradient flows into slopes, documents, prefixes and lengths.
  *   Operands are read with the strides of the views they are bound to; one whose last axis is not contiguous is copied.

@@ -17,6 +17,34 @@ def no_floors(monkeypatch):
     monkeypatch.setattr(oc, "FLOOR_WEIGHT", 0.0)
 
 
+def _without_lost_weights(c):
+    """tolerances for weights below 2^-125, which an fp32 exponential may flush to zero: all of what each contributes"""
+    ref = oc.attention_reference(c)
+    see, pos = oc.attention_sees(c)
+    extra = {n: np.zeros(x[1].shape) for n, x in ref.items()}
+    d, tk, h, g = c["q"].shape[3], c["k"].shape[1], c["q"].shape[2], c["k"].shape[2]
+    scale = 1 / np.sqrt(d) if c["scale"] is None else c["scale"]
+    for n in range(len(see)):
+        for m in range(h):
+            q, do = (c[x][n, :, m].astype(np.float64) for x in ("q", "do"))
+            k, v = (c[x][n, :, m // (h // g)].astype(np.float64) for x in "kv")
+            s = q @ k.T * scale
+            if c["cap"]:
+                s = c["cap"] * np.tanh(s / c["cap"])
+            if c["slopes"] is not None:
+                s = s - c["slopes"][m].astype(np.float64) * np.abs(pos[n][:, None] - np.arange(tk))
+            s = np.where(see[n], s, -np.inf)
+            p = np.exp(s - s.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            lost = np.where(p < 2.0 ** -125, p, 0)
+            ds = lost * (np.abs(do) @ np.abs(v).T + np.abs((do * (p @ v)).sum(1, keepdims=True))) * scale
+            extra["out"][n, :, m] = lost @ np.abs(v)
+            extra["dq"][n, :, m] = ds @ np.abs(k)
+            extra["dk"][n, :, m // (h // g)] += ds.T @ np.abs(q)
+            extra["dv"][n, :, m // (h // g)] += lost.T @ np.abs(do)
+    return {n: (x[0], x[1] + 2 * extra[n]) for n, x in ref.items()}
+
+
 def _side_by_side(d, ratio, tokens=260):
     """two documents in turn, token by token; one has keys, values and output gradients `ratio` times the other's, and queries
     larger by as much, so that the scores of both are of order one"""
@@ -88,13 +116,13 @@ def test_keys_of_little_weight(no_floors, d, few):
 
 
 @pytest.mark.parametrize("d", [64, 128, 40])
-@pytest.mark.parametrize("ratio", [2.0 ** -9, 2.0 ** -12, 2.0 ** -20])
+@pytest.mark.parametrize("ratio", [2.0 ** -9, 2.0 ** -12, 2.0 ** -20, 2.0 ** -40])
 def test_documents_token_by_token_in_one_tile(no_floors, d, ratio):
     c = _side_by_side(d, ratio)
     _tc_and_fp32(c)
 
 
-@pytest.mark.parametrize("kw", [dict(), dict(cap=4.0)])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=4.0), dict(slopes=True, causal=False), dict(cap=4.0, slopes=True)])
 @pytest.mark.parametrize("tq,tk,heads,d", [(700, 700, 2, 128), (130, 4000, 1, 64), (300, 300, 2, 96)])
 def test_rows_of_every_size(no_floors, kw, tq, tk, heads, d):
     """values and output gradients whose rows differ by up to 2^60, in every mixture; the middle case shares a tile's walk
@@ -107,7 +135,12 @@ def test_rows_of_every_size(no_floors, kw, tq, tk, heads, d):
         c[n] *= np.exp2(np.round(size)).astype(np.float32)[None, :, None, None]
     c["k"][:, ::7] *= np.float32(2.0 ** -14)
     c["q"][:, ::5] *= np.float32(2.0 ** -14)
-    _tc_and_fp32(c)
+    ref = _without_lost_weights(c)      # slopes of 1/2 over 4000 keys: weights down to e^-2000
+    for flags in (0, adb.devices.FLAG_SIMT_DOT):
+        dev = adb.devices.B200(0, flags=flags)
+        for n, x in oc.attention_run(dev, c).items():
+            oc.close(n, x, *ref[n])
+        dev.close()
 
 
 def test_rows_of_zeros_beside_others(no_floors):
@@ -118,3 +151,38 @@ def test_rows_of_zeros_beside_others(no_floors):
     _tc_and_fp32(c)
     c["do"][:], c["v"][:] = 0, 0
     _tc_and_fp32(c)
+
+
+@pytest.mark.parametrize("d", [64, 128, 160])
+@pytest.mark.parametrize("exponent", [-115, -105, 110, 117])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_values_near_the_ends_of_the_range(no_floors, d, exponent, mixed):
+    """finite values give finite results up to 2^117 times normal ones; `mixed`: among rows that are 2^-30 as large"""
+    c = oc.attention_case(1, 200, 200, 2, 2, d, seed=12)
+    if mixed and exponent > 0:
+        c["v"][:, ::3] *= np.float32(2.0 ** -30)
+    ref = oc.attention_reference(c)                  # for values of order one: out, dq and dk are linear in them
+    c["v"] *= np.float32(2.0 ** exponent)
+    for flags in (0, adb.devices.FLAG_SIMT_DOT):
+        dev = adb.devices.B200(0, flags=flags)
+        for n, x in oc.attention_run(dev, c).items():
+            size = 1.0 if n == "dv" else 2.0 ** exponent
+            # 200 terms of a few roundings each, which among the subnormals leave half of 2^-149, times a factor (q, k) below 8
+            oc.close(n, x.astype(np.float64) / size, ref[n][0], ref[n][1] + 200 * 4 * 8 * 2.0 ** -150 / size)
+        dev.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("exponent", [-110, -60, 60, 110])
+def test_large_queries_against_small_keys(no_floors, d, exponent):
+    """scores of order one out of operands at opposite ends of the range"""
+    c = oc.attention_case(1, 200, 200, 2, 2, d, seed=13)
+    ref = oc.attention_reference(c)
+    c["q"] *= np.float32(2.0 ** exponent)
+    c["k"] *= np.float32(2.0 ** -exponent)
+    for flags in (0, adb.devices.FLAG_SIMT_DOT):
+        dev = adb.devices.B200(0, flags=flags)
+        for n, x in oc.attention_run(dev, c).items():
+            size = {"dq": 2.0 ** -exponent, "dk": 2.0 ** exponent}.get(n, 1.0)
+            oc.close(n, x.astype(np.float64) / size, ref[n][0], ref[n][1] + 200 * 4 * 8 * 2.0 ** -150 / size)
+        dev.close()
