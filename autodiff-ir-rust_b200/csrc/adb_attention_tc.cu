@@ -1404,7 +1404,8 @@ cudaError_t grad_kernel(const GradArgs& f, dim3 grid, CUstream_st* stream) {
     auto go = [&](auto c, auto s) {
         constexpr bool CAP = decltype(c)::value, BIAS = decltype(s)::value;
         if constexpr (KEYS) {
-            // its warps share out the registers it is launched with: fewer than that sum would leave them waiting
+            // its warps share out the registers it is launched with: fewer than that sum would leave them waiting (the build
+            // checks the compiler's count; a library built another way is refused here)
             auto one = [&](auto kernel) {
                 cudaFuncAttributes attr;
                 cudaError_t e = cudaFuncGetAttributes(&attr, (const void*)kernel);
