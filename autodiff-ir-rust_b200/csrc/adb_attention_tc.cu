@@ -1342,8 +1342,8 @@ __global__ void __launch_bounds__(256) adb_attention_add(const float* part, floa
         out[i] = s;
     }
 }
-cudaError_t add_parts(const float* part, float* out, int64_t n, int64_t parts, CUstream_st* stream) {
-    adb_attention_add<<<unsigned(std::min<int64_t>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(part, out, n, int(parts));
+cudaError_t add_parts(const float* part, float* out, int64_t n, int64_t parts, int sm_count, CUstream_st* stream) {
+    adb_attention_add<<<unsigned(std::min<int64_t>((n + 255) / 256, int64_t(sm_count) * 8)), 256, 0, stream>>>(part, out, n, int(parts));
     return cudaGetLastError();
 }
 
@@ -1492,7 +1492,7 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
         e = P == 1 ? grad_kernel<1, false>(f, blocks, stream) : grad_kernel<2, false>(f, blocks, stream);
         n++;
         if (e == cudaSuccess && shares > 1) {
-            e = add_parts(f.dq, a.dq, size, shares, stream);
+            e = add_parts(f.dq, a.dq, size, shares, a.sm_count, stream);
             n++;
         }
     }
@@ -1508,7 +1508,7 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
         for (int i = 0; i < 2; i++) {
             float *part = i ? f.dv : f.dk, *out = i ? a.dv : a.dk;
             if (e == cudaSuccess && shares > 1 && out) {
-                e = add_parts(part, out, size, shares, stream);
+                e = add_parts(part, out, size, shares, a.sm_count, stream);
                 n++;
             }
         }
