@@ -27,7 +27,7 @@
 //   1. step positions increase in execution order (nested blocks lie between their parent and its successor);
 //   2. a buffer is alive at every step that touches it (external and whole-program buffers always are);
 //   3. buffers that are alive at the same time do not overlap in the arena;
-//   5. a dot product never writes into one of its own operands;
+//   5. a dot product or an operator never writes into one of its own operands;
 //   7. a collective over several buffers finds them side by side in the arena, in order, and covers exactly their span;
 //   6. the kernels that share one launch are independent: none writes a buffer that another reads or writes.
 // Returns an empty string or a description of the first violation.
@@ -46,6 +46,11 @@ static void step_buffers(const adb::Plan& plan, const adb::Step& s, std::vector<
     case Step::UPLOAD: case Step::ALLREDUCE:
         bufs = {s.buf};
         bufs.insert(bufs.end(), s.more_bufs.begin(), s.more_bufs.end());
+        break;
+    case Step::OPER:
+        for (auto& a : s.oper.in) if (a.buf >= 0) bufs.push_back(a.buf);
+        for (auto& a : s.oper.out) if (a.buf >= 0) bufs.push_back(a.buf);
+        if (s.oper.work >= 0) bufs.push_back(s.oper.work);
         break;
     case Step::WHILE: bufs = {s.cond_buf}; break;
     case Step::IF: for (auto& br : s.branches) bufs.push_back(br.cond_buf); break;
@@ -90,6 +95,14 @@ static std::string check_block(const adb::Plan& plan, const adb::StepBlock& blk,
         }
         if (s.kind == adb::Step::GEMM && (s.gemm.c == s.gemm.a || s.gemm.c == s.gemm.b || (s.gemm.out >= 0 && (s.gemm.out == s.gemm.a || s.gemm.out == s.gemm.b))))
             return "dot product at " + std::to_string(s.pos) + " writes into one of its operands";
+        if (s.kind == adb::Step::OPER)
+            for (size_t x = 0; x < s.oper.out.size(); x++) {
+                const int w = s.oper.out[x].buf;
+                bool clash = w >= 0 && w == s.oper.work;
+                for (auto& a : s.oper.in) clash = clash || (w >= 0 && a.buf == w) || (s.oper.work >= 0 && a.buf == s.oper.work);
+                for (size_t y = 0; y < x; y++) clash = clash || (w >= 0 && s.oper.out[y].buf == w);
+                if (clash) return "operator at " + std::to_string(s.pos) + " writes into one of its operands, its workspace or another result";
+            }
         step_buffers(plan, s, bufs);
         for (int b : bufs) {
             if (b < 0 || size_t(b) >= plan.bufs.size()) return "step at " + std::to_string(s.pos) + " names buffer " + std::to_string(b);

@@ -5,6 +5,7 @@
 // that is read before it is written, or that shares arena space with one that is still alive, shows up in the
 // results.
 #pragma once
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <limits>
@@ -163,6 +164,111 @@ struct PlanInterp {
         }
     }
 
+    // Operators of transformer layers, from their formulas in double precision.  Results and workspace are poisoned before an
+    // operand is read: a plan that lets them share memory shows up as NaN.
+    using Access = Step::Oper::Access;
+    const float* at(const Access& a, const std::vector<int64_t>& i) {
+        int64_t off = a.off;
+        for (size_t d = 0; d < i.size(); d++) off += i[d] * a.stride[d];
+        return ptr(a.buf, off);
+    }
+    void run_oper(const Step::Oper& o) {
+        auto poison = [&](int buf) { if (buf >= 0) std::fill_n(ptr(buf), plan.bufs[size_t(buf)].numel, std::numeric_limits<float>::quiet_NaN()); };
+        for (auto& a : o.out) poison(a.buf);
+        poison(o.work);
+        auto has = [&](size_t i) { return o.in[i].buf >= 0; };
+        auto flat = [&](size_t i) { return ptr(o.in[i].buf, o.in[i].off); };
+        auto put = [&](size_t k, int64_t i, double v) { if (o.out[k].buf >= 0) ptr(o.out[k].buf)[i] = float(v); };
+        const auto& d = o.dims;
+        if (o.op == OP_RMS_NORM || o.op == OP_RMS_NORM_GRAD) {
+            const bool grad = o.op == OP_RMS_NORM_GRAD;
+            std::vector<double> dg(size_t(d[1]), 0.0);
+            for (int64_t r = 0; r < d[0]; r++) {
+                std::vector<double> h;
+                double s = 0, along = 0;
+                for (int64_t c = 0; c < d[1]; c++) {
+                    h.push_back(*at(o.in[0], {r, c}) + (!grad && has(2) ? double(*at(o.in[2], {r, c})) : 0.0));
+                    s += h.back() * h.back();
+                }
+                const double inv = 1 / std::sqrt(s / double(d[1]) + o.reals[0]);
+                for (int64_t c = 0; c < d[1] && grad; c++) along += double(*at(o.in[2], {r, c})) * flat(1)[c] * h[size_t(c)] * inv / double(d[1]);
+                for (int64_t c = 0; c < d[1]; c++) {
+                    const double n = h[size_t(c)] * inv;
+                    if (!grad) {
+                        put(0, r * d[1] + c, n * flat(1)[c]);
+                        put(1, r * d[1] + c, h[size_t(c)]);
+                        continue;
+                    }
+                    const double dy = *at(o.in[2], {r, c});
+                    dg[size_t(c)] += dy * n;
+                    put(0, r * d[1] + c, inv * (dy * flat(1)[c] - n * along) + (has(3) ? double(*at(o.in[3], {r, c})) : 0.0));
+                }
+            }
+            for (int64_t c = 0; c < d[1] && grad; c++) put(1, c, dg[size_t(c)]);
+        } else if (o.op == OP_ROTARY) {
+            for (int64_t b = 0; b < d[0]; b++)
+                for (int64_t t = 0; t < d[1]; t++)
+                    for (int64_t h = 0; h < d[2]; h++)
+                        for (int64_t c = 0; c < d[3]; c++) {
+                            const int64_t to = ((b * d[1] + t) * d[2] + h) * d[3] + c, P = d[4];
+                            const double x = *at(o.in[0], {b, t, h, c});
+                            if (c >= 2 * P) { put(0, to, x); continue; }
+                            const int64_t p = o.ints[0] ? c / 2 : c % P;
+                            const bool second = o.ints[0] ? c & 1 : c >= P;
+                            const int64_t mate = o.ints[0] ? c ^ 1 : second ? c - P : c + P;
+                            const double pos = has(2) ? double(*at(o.in[2], {b, t})) : double(o.ints[2] + t);
+                            const double turns = pos * (double(flat(1)[p]) + flat(1)[P + p]), angle = 2 * M_PI * (turns - std::floor(turns));
+                            const double sn = std::sin(angle) * (o.ints[1] ? -1 : 1) * (second ? 1 : -1);
+                            put(0, to, o.reals[0] * (x * std::cos(angle) + *at(o.in[0], {b, t, h, mate}) * sn));
+                        }
+        } else {
+            const bool grad = o.op == OP_ATTENTION_GRAD, causal = o.ints[0] != 0;
+            const int64_t B = d[0], Tq = d[1], Tk = d[2], H = d[3], G = d[4], D = d[5];
+            const double scale = o.reals[0], cap = o.reals[1];
+            std::vector<double> dk(size_t(B * Tk * G * D), 0.0), dv(dk);
+            auto count = [&](size_t i, int64_t b) { const double x = flat(i)[b]; return x > 0 ? int64_t(std::min(x, double(Tk))) : int64_t(0); };
+            for (int64_t b = 0; b < B; b++)
+                for (int64_t h = 0; h < H; h++)
+                    for (int64_t i = 0; i < Tq; i++) {
+                        const int64_t g = h / (H / G), n = has(6) ? count(6, b) : Tk, prefix = has(5) ? count(5, b) : 0, pos = i + n - Tq;
+                        const float* doc = has(4) ? flat(4) + b * Tk : nullptr;
+                        std::vector<double> s(size_t(Tk), -INFINITY), bend(size_t(Tk), 1.0), out(size_t(D), 0.0), dq(out);
+                        double top = -INFINITY, sum = 0, along = 0;
+                        for (int64_t j = 0; j < n; j++) {
+                            if (((causal || has(6)) && pos < 0) || (causal && j > pos && j >= prefix)) continue;
+                            if (doc && !(doc[j] >= 0 && doc[pos] == doc[j])) continue;
+                            double x = 0;
+                            for (int64_t c = 0; c < D; c++) x += double(*at(o.in[0], {b, i, h, c})) * *at(o.in[1], {b, j, g, c});
+                            x *= scale;
+                            if (cap > 0) { const double t = std::tanh(x / cap); x = cap * t; bend[size_t(j)] = 1 - t * t; }
+                            if (has(3)) x -= double(flat(3)[h]) * std::abs(double(pos - j));
+                            s[size_t(j)] = x;
+                            top = std::max(top, x);
+                        }
+                        for (double x : s) if (x > -INFINITY) sum += std::exp(x - top);
+                        const int64_t row = (b * H + h) * Tq + i;
+                        if (!grad) put(1, row, sum > 0 ? (top + std::log(sum)) / std::log(2.0) : -INFINITY);
+                        for (int64_t c = 0; c < D && grad; c++) along += double(*at(o.in[7], {b, i, h, c})) * *at(o.in[9], {b, i, h, c});
+                        for (int64_t j = 0; j < Tk; j++) {
+                            if (!(s[size_t(j)] > -INFINITY)) continue;
+                            const double p = grad ? std::exp2(s[size_t(j)] / std::log(2.0) - flat(8)[row]) : std::exp(s[size_t(j)] - top) / sum;
+                            double dp = 0;
+                            for (int64_t c = 0; c < D && grad; c++) dp += double(*at(o.in[9], {b, i, h, c})) * *at(o.in[2], {b, j, g, c});
+                            const double ds = p * (dp - along) * bend[size_t(j)] * scale;
+                            for (int64_t c = 0; c < D; c++) {
+                                const size_t key = size_t(((b * Tk + j) * G + g) * D + c);
+                                if (!grad) { out[size_t(c)] += p * *at(o.in[2], {b, j, g, c}); continue; }
+                                dq[size_t(c)] += ds * *at(o.in[1], {b, j, g, c});
+                                dk[key] += ds * *at(o.in[0], {b, i, h, c});
+                                dv[key] += p * *at(o.in[9], {b, i, h, c});
+                            }
+                        }
+                        for (int64_t c = 0; c < D; c++) put(0, ((b * Tq + i) * H + h) * D + c, grad ? dq[size_t(c)] : out[size_t(c)]);
+                    }
+            for (size_t i = 0; i < dk.size() && grad; i++) { put(1, int64_t(i), dk[i]); put(2, int64_t(i), dv[i]); }
+        }
+    }
+
     void run_step(const Step& s) {
         switch (s.kind) {
         case Step::ELW: case Step::REDUCE: {
@@ -240,6 +346,7 @@ struct PlanInterp {
             if (!taken && s.else_body) run_block(*s.else_body);
             break;
         }
+        case Step::OPER: run_oper(s.oper); break;
         case Step::EXIT: exited = true; break;
         }
     }
