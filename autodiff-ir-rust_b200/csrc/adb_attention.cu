@@ -347,8 +347,9 @@ bool launch_tiles(K kernel, const AttentionArgs& a, const Vec& vec, int T, int64
 }  // namespace
 
 int attention_launch(const AttentionArgs& a, CUstream_st* stream, std::string& err) {
-    if (attention_uses_tc(a.s)) return attention_tc_launch(a, stream, err);
-    if (a.s.tq < 64 && fits16(a.k, a.s.dim) && fits16(a.v, a.s.dim)) return attention_split_launch(a, stream, err);
+    const bool few = a.s.tq < 64 && fits16(a.k, a.s.dim) && fits16(a.v, a.s.dim);
+    if (attention_uses_tc(a.s) && !(few && attention_prefers_rows(a.s))) return attention_tc_launch(a, stream, err);
+    if (few) return attention_split_launch(a, stream, err);
     const int dim = int(a.s.dim), ld = padded(dim);
     const Vec vec{fits16(a.q, dim), fits16(a.k, dim), fits16(a.v, dim), false, false};
     const size_t smem = (size_t(3) * 64 * ld + 64 * 68) * 4;

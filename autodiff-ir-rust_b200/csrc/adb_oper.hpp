@@ -78,11 +78,17 @@ constexpr int64_t ATTENTION_TC_MAX_DIM = 128, ATTENTION_TC_TILE = 128;
 constexpr int ATTENTION_GAVE_UP = 33;   // first code of a bounded wait of theirs that ran out
 inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
 // With few queries a tile of 128 is mostly padding and the keys are worth reading once only: adb_attention_decode.cu.  From
-// 8 queries on the tile is the faster one all the same (8 queries of 16 heads over 4 against 8000 keys: 50 us against 94;
-// 15 of 32 heads over 32 against 2000: 59 against 90).
+// 8 queries on the tile can be the faster one all the same.
 inline bool attention_uses_tc(const AttentionShape& s) {
     return !s.cuda_cores && s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 8 && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
+// The tile costs making images of the cache (12 bytes moved for 4) and a tile for each head, the kernel for few queries as much
+// again for every 8 rows (queries of the heads that share a key head): it is the better one up to 8 rows of 128 elements.
+// Tile against the other, us: 8 rows of 128, 8 x 16384 keys of 32 heads 2107 / 1176, 2000 keys 61 / 55 (4 x 2000: 156 / 169);
+// 8 rows of 64, 128 x 512 of 16 heads 427 / 149, 300 of 8 heads 22 / 16; 12 rows of 64, 256 x 200 of 16 heads 502 / 333; 16
+// rows of 32, 16 x 4000 of 16 heads 353 / 160.  More rows: 15 of 128, 2000 of 32 heads 62 / 88, 8 x 2000 291 / 375; 32 of 128,
+// 8000 of 4 key heads 51 / 92, 32 x 16384 of 8 key heads 3539 / 4371; 24 of 64, 8 x 4000 of 32 heads 365 / 356.
+inline bool attention_prefers_rows(const AttentionShape& s) { return s.tq < 64 && s.heads / s.kv_heads * s.tq * s.dim <= 1024; }
 // How many blocks share one tile's walk over the other side when there are fewer tiles than SMs: as many as fill the SMs,
 // each with at least `least` steps.  Their results are added (or joined) in order by a kernel of their own.
 inline int64_t attention_shares(int64_t tiles, int64_t steps, int64_t least, int sm_count) {
@@ -111,11 +117,13 @@ inline int64_t attention_ranges(const AttentionShape& s, int sm_count) {
     return (s.tk + keys - 1) / keys;
 }
 inline int64_t attention_workspace(const AttentionShape& s, int sm_count) {
-    if (!attention_uses_tc(s)) return s.batch * s.tq * s.heads * attention_ranges(s, sm_count) * (s.dim + 2);
+    const int64_t parts = s.batch * s.tq * s.heads * attention_ranges(s, sm_count) * (s.dim + 2);   // of ranges of keys
+    if (!attention_uses_tc(s)) return parts;
     // images of keys and values, their scales by tile and by row, document numbers; each part begins on a 256-byte boundary
     const int64_t tiles = attention_tc_tiles(s.tk), n = s.batch * s.kv_heads * tiles, shares = attention_forward_shares(s, sm_count);
-    return 2 * (n * (attention_panels(s.dim) * 8192 + 1 + ATTENTION_TC_TILE) + 128) + 4 * s.batch * tiles + 64 +
-           (shares > 1 ? s.batch * s.tq * s.heads * shares * (s.dim + 2) : 0);
+    const int64_t images = 2 * (n * (attention_panels(s.dim) * 8192 + 1 + ATTENTION_TC_TILE) + 128) + 4 * s.batch * tiles + 64 +
+                           (shares > 1 ? s.batch * s.tq * s.heads * shares * (s.dim + 2) : 0);
+    return attention_prefers_rows(s) ? std::max(images, parts) : images;   // (which of the two also depends on the operands' strides)
 }
 // The gradient takes them whatever the count of queries: the CUDA-core kernels' tiles of 64 are just as empty.
 inline bool attention_grad_uses_tc(const AttentionShape& s) {

@@ -424,3 +424,24 @@ def test_result_over_its_operand():
         oc.close("x", n, *ref["y"])
         again = oc.norm_reference(dict(x, x=n))
         oc.close("y", y, *again["y"])
+
+
+@pytest.mark.parametrize("b,tq,tk,h,g,d,kw", [
+    (3, 8, 900, 4, 4, 128, dict(lengths=[900, 5, 400])), (2, 16, 700, 3, 3, 64, dict(cap=6.0, slopes=True)), (2, 31, 300, 1, 1, 32, {}),
+    (2, 8, 500, 8, 2, 32, dict(docs=_docs(2, 500, 90, 30))), (1, 63, 200, 2, 2, 16, dict(prefix=[30])), (2, 9, 333, 2, 2, 100, dict(causal=False)),
+    (1, 9, 400, 2, 2, 128, {}), (2, 10, 300, 1, 1, 90, {})])
+def test_from_8_queries_on(b, tq, tk, h, g, d, kw):
+    """either side of the rule between tiles and rows; the last two: too many rows, and a head size that rows of 16 bytes do not fit"""
+    c = oc.attention_case(b, tq, tk, h, g, d, seed=tq, **kw)
+    oc.attention_check(oc.attention_run(b200(), c, grad=False), c)
+
+
+def test_few_queries_of_operands_off_the_16_byte_grid():
+    """keys and values that start 4 bytes behind a boundary: the tile takes them although rows would be preferred"""
+    c = oc.attention_case(1, 8, 300, 2, 2, 64, seed=3)
+    oc.start(b200())
+    wide = {n: np.concatenate([np.zeros(c[n].shape[:3] + (1,), np.float32), c[n]], 3) for n in "kv"}
+    k, v = (oc.leaf(wide[n]).r(range(1, 65), 3) for n in "kv")
+    out = ad.attention(oc.leaf(c["q"]), k, v)
+    got = oc.finish({"out": out.forward()})
+    oc.attention_check(got, c)
