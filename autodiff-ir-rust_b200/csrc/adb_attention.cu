@@ -1,6 +1,6 @@
 // Attention and its gradient on the CUDA cores: the general kernels, for every head size, stride and mask.  They serve heads
-// of more than 128 elements, short sequences (fewer than 64 keys; few queries over keys that 16-byte accesses do not fit)
-// and batches of more than 65535 heads.
+// of more than 128 elements, short sequences (fewer than 64 keys), few queries over keys off the 16-byte grid, batches of
+// more than 65535 heads, and devices made with ADB_FLAG_SIMT_DOT.
 //
 //   forward   o = sum_j p_j v_j,  p = softmax of the scores; one pass over the keys with the running maximum and sum
 //   gradient  p_ij = exp2(s_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i) bend_ij scale

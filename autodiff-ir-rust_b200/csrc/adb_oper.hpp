@@ -78,9 +78,10 @@ constexpr int64_t ATTENTION_TC_MAX_DIM = 128, ATTENTION_TC_TILE = 128;
 constexpr int ATTENTION_GAVE_UP = 33;   // first code of a bounded wait of theirs that ran out
 inline int attention_panels(int64_t dim) { return dim <= 64 ? 1 : 2; }
 // With few queries a tile of 128 is mostly padding and the keys are worth reading once only: adb_attention_decode.cu.  From
-// 8 queries on the tile can be the faster one all the same.
+// 8 queries on the tile can be the faster one all the same, and it takes what that kernel's 16-byte accesses do not fit: one query of
+// 32 x 16384 keys, 32 heads over 8 of 126, 3.6 ms against 39 in the general kernel; 1025 keys, 8 over 2 of 62: 32 us / 188.
 inline bool attention_uses_tc(const AttentionShape& s) {
-    return !s.cuda_cores && s.dim <= ATTENTION_TC_MAX_DIM && s.tq >= 8 && s.tk >= 64 && s.batch * s.heads <= 65535;
+    return !s.cuda_cores && s.dim <= ATTENTION_TC_MAX_DIM && (s.tq >= 8 || s.dim % 4) && s.tk >= 64 && s.batch * s.heads <= 65535;
 }
 // The tile costs making images of the cache (12 bytes moved for 4) and a tile for each head, the kernel for few queries as much
 // again for every 8 rows (queries of the heads that share a key head): it is the better one up to 8 rows of 128 elements.

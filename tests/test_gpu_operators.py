@@ -445,3 +445,11 @@ def test_few_queries_of_operands_off_the_16_byte_grid():
     out = ad.attention(oc.leaf(c["q"]), k, v)
     got = oc.finish({"out": out.forward()})
     oc.attention_check(got, c)
+
+
+@pytest.mark.parametrize("b,tq,tk,h,g,d,kw", [
+    (2, 1, 1025, 8, 2, 62, dict(slopes=True)), (3, 1, 700, 4, 4, 126, dict(lengths=[700, 0, 65])), (1, 3, 64, 2, 1, 5, {}),
+    (2, 7, 500, 6, 3, 99, dict(docs=_docs(2, 500, 120, 40), cap=3.0)), (1, 1, 9000, 2, 2, 30, dict(causal=False))])
+def test_few_queries_of_odd_head_sizes(b, tq, tk, h, g, d, kw):
+    c = oc.attention_case(b, tq, tk, h, g, d, seed=d, **kw)
+    oc.attention_check(oc.attention_run(b200(), c, grad=False), c)
