@@ -963,7 +963,9 @@ def rotary(x: Tensor, table: Tensor, positions: Tensor = None, offset: int = 0, 
     """Turns the first 2 P elements of every head of `x` [batch, tokens, heads, head size] by angles that grow with the
     token's position: `positions` ([tokens] or [batch, tokens], whole numbers) or offset + token.  `table` [2, P] holds
     each pair's frequency in whole turns per position as the sum of two floats (`nn.Rotary` makes it).  A pair is two
-    neighbours (`interleaved`) or elements i and P + i.  No gradient flows into the table and the positions."""
+    neighbours (`interleaved`) or elements i and P + i.  `offset` is part of the program: a decoding loop, whose position
+    changes with every token, hands `positions` over instead, so that one program serves all of its steps.  No gradient flows
+    into the table and the positions."""
     d, t = x.dim(), table.dim()
     if len(d) != 4:
         raise ValueError("rotary needs [batch, tokens, heads, head size]")

@@ -18,6 +18,11 @@ namespace adb {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // whole number of tokens out of a float that a caller filled (NaN and negative numbers: none)
 __device__ __forceinline__ int token_count(const float* p, int64_t b, int most) {
     return p ? int(fminf(fmaxf(__ldg(p + b), 0.f), float(most))) : most;
@@ -40,7 +45,7 @@ struct Sight {
     __device__ __forceinline__ bool query_used(int pos) const {
         return !(hide_before && pos < 0) && pos < n && !(docs && !(docs[pos] >= 0.f));
     }
-    // first key that no query up to `last_pos` sees, first query position that sees key j
+    // the first key that no query up to `last_pos` sees
     __device__ __forceinline__ int keys_end(int last_pos) const {
         return causal ? min(n, max(last_pos + 1, prefix)) : n;
     }
@@ -51,7 +56,7 @@ struct Sight {
 };
 
 // tanh to fp32 accuracy from one ex2 and one reciprocal; near zero, where 1 - 2 / (e + 1) cancels, its odd series (the
-// first omitted term is below 2e-8 of x at 0.3)
+// first omitted term, 1382/155925 x^10 of x, is 5.2e-8 at 0.3: less than an fp32 rounding)
 __device__ __forceinline__ float tanh_exact(float x) {
     const float e = exp2f(2.f * LOG2E * fabsf(x));
     const float far = copysignf(1.f - __fdividef(2.f, e + 1.f), x);

@@ -24,11 +24,6 @@ __host__ __device__ constexpr int step_keys(int nv) { return nv == 1 ? 4 : nv ==
 __host__ __device__ constexpr int stage_quads(int nv) { return 2 * step_keys(nv) * nv * THREADS; }
 static_assert(ATTENTION_SPLIT_STEP == GROUPS * 4, "keys a block takes at a time, at most");
 
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 // Sums of R numbers over eight lanes, each lane left with the one whose row it owns (8 / R lanes own a row together): a lane
 // that gives half of its numbers away at each exchange needs R - 1 + log2(8 / R) of them instead of 3 R, and what follows
 // from a sum (the score, its exponential) is worked out once instead of eight times.

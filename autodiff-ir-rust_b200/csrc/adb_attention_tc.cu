@@ -4,9 +4,13 @@
 // per element each way), so that the kernel proper fetches ready operands by bulk copies however the caller's tensors
 // are strided.
 //
-// Measured on 2 x 4096 tokens, 16 heads of 128, causal: images 46 us (5.8 TB/s), forward
-// 389 us, images of the gradient's four operands 111 us, dq 686 us, dk and dv 908 us; at the tensor cores' own rate the
-// products take 190, 285 and 380 us.  Error against 64 bits 8e-7 of a result's norm; fp32 products in cuBLAS: 1.7e-6.
+// Rows of an image are held in units of their own where they differ much in size; every loop over tiles exists a second time
+// for that (BY_ROWS), so that a result is as exact as what it is made of, whatever stands beside it.
+//
+// Measured on 2 x 4096 tokens, 16 heads of 128, causal: images 49 us (5.5 TB/s), forward 397 us, images of the gradient's
+// four operands 118 us, dq 679 us, dk and dv 973 + 15 us; at the tensor cores' own rate the products take 190, 285 and 380 us.
+// With rows that differ by up to 2^40 forward and gradient take 2.55 ms instead of 2.18.  Error against 64 bits 8e-7 of a
+// result's norm; fp32 products in cuBLAS: 1.7e-6.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -25,15 +29,9 @@ constexpr int KT = 128;                 // keys of a tile
 constexpr int PARTS = 4;
 constexpr int SOFTMAX_WARPS = 4 * PARTS, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
-// Weights of a tile are kept in units that make the row's largest 2^15: half of fp16's smallest step, 2^-25, is 2^-40 of it,
-// and a weight of 2^-18 of the row's largest still has both halves' 22 bits.
+// Weights of a tile are kept in units that bring the row's largest into (2^14, 2^15]: half of fp16's smallest step is at most
+// 2^-39 of it, and a weight of 2^-17 of the largest still has both halves' 22 bits.
 constexpr float P_SHIFT = 15.f;
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 
 // ------------------------------------------------------------------------------------------ images
 struct ImageJob {
@@ -1330,10 +1328,6 @@ __global__ void __launch_bounds__(KEY_THREADS, 1) adb_attention_tc_dkv(const Gra
     if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 
-bool fits16(const Strided4& t, int64_t dim) {
-    return (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && dim % 4 == 0 && t.bs % 4 == 0 && t.ts % 4 == 0 && t.hs % 4 == 0;
-}
-
 // out[i] = sum of `parts` numbers n apart, in order
 __global__ void __launch_bounds__(256) adb_attention_add(const float* part, float* out, int64_t n, int parts) {
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
@@ -1363,7 +1357,7 @@ cudaError_t forward(const ForwardArgs& f, dim3 grid, CUstream_st* stream) {
     return bias ? launch(adb_attention_tc<P, false, true>, grid, THREADS, smem, stream, f) : launch(adb_attention_tc<P, false, false>, grid, THREADS, smem, stream, f);
 }
 
-bool aligned_rows(const float* p, int64_t dim) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && dim % 4 == 0; }
+bool aligned_rows(const float* p, int64_t dim) { return aligned16(p) && dim % 4 == 0; }
 
 // the workspace, cut up
 struct Cut {
@@ -1504,7 +1498,7 @@ int attention_tc_grad_launch(const AttentionArgs& a, CUstream_st* stream, std::s
         f.out_vec = aligned_rows(f.dk, s.dim) && aligned_rows(f.dv, s.dim);
         const dim3 blocks(unsigned(s.batch * s.kv_heads * k_tiles), unsigned(shares));
         e = P == 1 ? grad_kernel<1, true>(f, blocks, stream) : grad_kernel<2, true>(f, blocks, stream);
-        n++;
+        n += 2;
         for (int i = 0; i < 2; i++) {
             float *part = i ? f.dv : f.dk, *out = i ? a.dv : a.dk;
             if (e == cudaSuccess && shares > 1 && out) {

@@ -6,7 +6,8 @@
 // Both are bound by HBM: 16 bytes per element forward (x, r in; y, h out), 16 backward (h, dy, dh in; dx out).  A row is
 // read once: a warp (rows of up to 1024 elements) or a block holds its share of the row in registers while the sums run
 // through shuffles and, across warps, shared memory in a fixed order.  Sums are fp32: a thread adds at most 32 products
-// one after another, the rest is a tree.
+// one after another (a 1024th of the row where rows are wider than registers hold), the rest is a tree; dg adds a block's
+// rows one after another, then the blocks.
 //
 // Measured: 65536 rows of 1024, forward and gradient, 2.15 GB in 340 us = 6.3 TB/s, 0.97 of the copy rate.  2001 rows of 5003
 // (no 16-byte access fits, a block a row): forward 31 us = 5.2 TB/s, gradient about 50 us = 3.2 TB/s, bound by the two
@@ -230,8 +231,6 @@ __global__ void __launch_bounds__(1024) adb_column_sums(const float* part, float
     const int64_t own = int64_t(blockIdx.x) * 32 + y;
     if (x == 0 && own < width) out[own] = s;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int launched(int n, std::string& err) {
     const cudaError_t e = cudaGetLastError();

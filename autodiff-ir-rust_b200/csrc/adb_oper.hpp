@@ -54,10 +54,15 @@ struct AttentionShape {
     int64_t batch = 0, tq = 0, tk = 0, heads = 0, kv_heads = 0, dim = 0;
     bool cuda_cores = false;   // fp32 products only (ADB_FLAG_SIMT_DOT)
 };
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 struct Strided4 {   // [batch, tokens, heads, dim], dim contiguous
     const float* p = nullptr;
     int64_t bs = 0, ts = 0, hs = 0;
 };
+// rows that 16-byte accesses fit
+inline bool fits16(const Strided4& t, int64_t dim) {
+    return t.p && aligned16(t.p) && dim % 4 == 0 && t.bs % 4 == 0 && t.ts % 4 == 0 && t.hs % 4 == 0;
+}
 struct AttentionArgs {
     AttentionShape s;
     Strided4 q, k, v, out, dout;            // out (as an operand) and dout: gradient only

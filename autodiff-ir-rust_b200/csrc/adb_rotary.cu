@@ -85,8 +85,6 @@ __global__ void __launch_bounds__(THREADS) adb_rotary(const RotaryArgs a, const 
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace
 
 int rotary_launch(const RotaryArgs& a, CUstream_st* stream, std::string& err) {
