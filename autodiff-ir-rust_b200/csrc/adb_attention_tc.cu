@@ -29,8 +29,8 @@ constexpr int KT = 128;                 // keys of a tile
 constexpr int PARTS = 4;
 constexpr int SOFTMAX_WARPS = 4 * PARTS, MMA_WARP = SOFTMAX_WARPS, LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
-// Weights of a tile are kept in units that bring the row's largest into (2^14, 2^15]: half of fp16's smallest step is at most
-// 2^-39 of it, and a weight of 2^-17 of the largest still has both halves' 22 bits.
+// Weights of a tile are kept in units that make the row's largest 2^15: half of fp16's smallest step, 2^-25, is 2^-40 of it,
+// and a weight of 2^-18 of the row's largest still has both halves' 22 bits.
 constexpr float P_SHIFT = 15.f;
 
 // ------------------------------------------------------------------------------------------ images
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
         constexpr bool BY_ROWS = decltype(units)::value;
         const ScoreOf score(a, h);
         [[maybe_unused]] const float cap2 = score.cap2, slope2 = score.slope2;
-        float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_before = 0.f;
+        float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_first = 1.f, v_before = 0.f;
 #pragma unroll
         for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
         bool ok = true;
@@ -531,6 +531,9 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(o_empty);
+            if (v_first != 1.f)
+#pragma unroll
+                for (int c = 0; c < SHARE; c++) r[c] = __float_as_uint(__uint_as_float(r[c]) * v_first);
 #pragma unroll
             for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), v_before, acc[c] * keep);
             return true;
@@ -592,9 +595,8 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
 #pragma unroll
             for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
             if (!ok) break;
-            // Weights in units of the tile's own largest, sums and results in units of the largest so far, both rounded up
-            // to powers of two: what is rescaled keeps its bits, and a unit of values near 2^-126 is exact among the subnormals.
-            const float tile_top = ceilf(row_max(cell, row)), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
+            // weights in units of the tile's own largest, sums and results in units of the largest so far
+            const float tile_top = row_max(cell, row), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
             const float from = (tile_top == -INFINITY ? 0.f : tile_top) - P_SHIFT;
             const float fade = ex2(m - base), unit = ex2(tile_top - base - P_SHIFT);
             m = top;
@@ -622,7 +624,10 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             l = fmaf(l, fade, ((sums[0] + sums[1]) + (sums[2] + sums[3])) * unit);
             if (i > 0) ok = drain(i - 1);
             keep = fade;
-            v_before = v_scale * unit;
+            // (two steps where the product would be a subnormal number and lose bits of its own)
+            const bool tiny = v_scale < 0x1p-100f;
+            v_first = tiny ? unit : 1.f;
+            v_before = tiny ? v_scale : v_scale * unit;
         }
         if (ok && i > 0) ok = drain(i - 1);
         float* cell = exchange + (i & 1) * PARTS * ROWS;   // (the last tile's may still be being read)

@@ -186,3 +186,12 @@ def test_large_queries_against_small_keys(no_floors, d, exponent):
             size = {"dq": 2.0 ** -exponent, "dk": 2.0 ** exponent}.get(n, 1.0)
             oc.close(n, x.astype(np.float64) / size, ref[n][0], ref[n][1] + 200 * 4 * 8 * 2.0 ** -150 / size)
         dev.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_single_key_has_a_weight_of_exactly_one(d):
+    """documents of one token each: the output is the value to the halves' 22 bits, as the one score is its own maximum"""
+    c = oc.attention_case(1, 200, 200, 2, 2, d, seed=21, docs=np.arange(200)[None], scale=2.0)
+    got = oc.attention_run(adb.devices.B200(0), c, grad=False)["out"]
+    # hi + lo leave half of 2^-21 of a value and 2^-39 of its row's largest
+    oc.close("out", got, c["v"], 2.0 ** -22 * np.abs(c["v"]) + 2.0 ** -39 * np.abs(c["v"]).max(-1, keepdims=True) + oc.U * np.abs(c["v"]))
