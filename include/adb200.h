@@ -82,6 +82,8 @@ typedef enum adb_status {
  *                      causal: j <= p or j < prefix; documents: the numbers at p and j agree and are not negative.
  *                      Causal or with lengths, a query with p < 0 sees nothing.  A query that sees nothing: out 0, lse -inf.
  *                      Lengths and prefixes are cut to [0, Tk] and to whole numbers (NaN: 0).
+ *                      Heads of up to 128 elements run on the tensor cores where that is faster, operands as sums of two fp16
+ *                      halves: off by 2^-22 of a value and 2^-39 of its row's largest (ADB_FLAG_SIMT_DOT: fp32 products).
  *                      Results are finite for finite operands as long as sums of |v| over the keys stay within fp32's range.
  *                      Rows behind a sequence's length and rows of padding are not read; an infinity or a NaN in any
  *                      other row may reach every query of its sequence and head.
