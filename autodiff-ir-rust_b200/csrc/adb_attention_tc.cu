@@ -261,15 +261,15 @@ __device__ __forceinline__ bool units_by_row(const float* one, const float* othe
 }
 // What a row's unit is multiplied with to give its largest magnitude, within a factor of two.
 constexpr float ROW_TOP = 16384.f;
+// a factor that is finite, so that zeros stay zeros
+__device__ __forceinline__ float in_range(float f) { return fmaxf(fminf(f, 3.4e38f), -3.4e38f); }
 // A product of units that may lie at opposite ends of the range: x * a row's factor * a column's, the factor below one first.
 // Only a product that is out of range itself, or whose factors are 2^186 apart, leaves it.
 struct RowFactor {
     float before, after;
-    __device__ __forceinline__ explicit RowFactor(float f) : before(fabsf(f) < 1.f ? f * (1.f / ROW_TOP) : 1.f / ROW_TOP), after(fabsf(f) < 1.f ? ROW_TOP : f * ROW_TOP) {}
+    __device__ __forceinline__ explicit RowFactor(float f) : before(fabsf(f) < 1.f ? f * (1.f / ROW_TOP) : 1.f / ROW_TOP), after(fabsf(f) < 1.f ? ROW_TOP : in_range(f * ROW_TOP)) {}
     __device__ __forceinline__ float operator()(float x, float column) const { return x * before * column * after; }
 };
-// one factor for a tile: finite, so that zeros stay zeros
-__device__ __forceinline__ float in_range(float f) { return fmaxf(fminf(f, 3.4e38f), -3.4e38f); }
 // a tile's columns times the units of the rows they stand for (16-byte boundary) and the row's own factor
 template <int N>
 __device__ __forceinline__ void times_rows(uint32_t (&r)[N], const float* units, const RowFactor& own) {

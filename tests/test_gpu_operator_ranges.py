@@ -195,3 +195,18 @@ def test_a_single_key_has_a_weight_of_exactly_one(d):
     got = oc.attention_run(adb.devices.B200(0), c, grad=False)["out"]
     # hi + lo leave half of 2^-21 of a value and 2^-39 of its row's largest
     oc.close("out", got, c["v"], 2.0 ** -22 * np.abs(c["v"]) + 2.0 ** -39 * np.abs(c["v"]).max(-1, keepdims=True) + oc.U * np.abs(c["v"]))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_queries_of_zeros_have_scores_of_zero(d, mixed):
+    """whatever the keys and the scale are: the product of their units is out of range, the scores are not"""
+    c = oc.attention_case(1, 150, 150, 2, 2, d, seed=22, scale=1000.0)
+    c["q"][:], c["k"] = 0, c["k"] * np.float32(2.0 ** 122)
+    if mixed:
+        c["do"][:, ::3] *= np.float32(2.0 ** -30)
+    got = oc.attention_run(adb.devices.B200(0), c)
+    ref = oc.attention_reference(dict(c, k=c["k"] * np.float32(2.0 ** -122), scale=1.0))
+    for n in ("out", "dv"):
+        oc.close(n, got[n], *ref[n])
+    assert not got["dk"].any()
