@@ -515,147 +515,147 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc(const ForwardArgs
             row_sync(quad);
         }
         auto arithmetic = [&](auto units) {
-        constexpr bool BY_ROWS = decltype(units)::value;
-        const ScoreOf score(a, h);
-        [[maybe_unused]] const float cap2 = score.cap2, slope2 = score.slope2;
-        float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_first = 1.f, v_before = 0.f;
+            constexpr bool BY_ROWS = decltype(units)::value;
+            const ScoreOf score(a, h);
+            [[maybe_unused]] const float cap2 = score.cap2, slope2 = score.slope2;
+            float acc[SHARE], m = -INFINITY, l = 0.f, keep = 0.f, v_first = 1.f, v_before = 0.f;
 #pragma unroll
-        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-        bool ok = true;
-        auto drain = [&](int i) {   // O of tile i
-            if (!bar_wait_warp(o_full, i & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
-            fence_after();
-            uint32_t r[SHARE];
-            tmem_load(lanes + 384 + part * SHARE, r);
-            tmem_wait_load();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(o_empty);
-            if (v_first != 1.f)
-#pragma unroll
-                for (int c = 0; c < SHARE; c++) r[c] = __float_as_uint(__uint_as_float(r[c]) * v_first);
-#pragma unroll
-            for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), v_before, acc[c] * keep);
-            return true;
-        };
-        int i = 0;
-        const int pos_first = q0 + sight.shift;
-        int t = walk.first();
-        bool docs_next = t >= 0 && !walk.one_document(t);
-        float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
-        for (int next; t >= 0; t = next, i++) {
-            const int k0 = t * KT + KEYS * part;
-            const float mul = BY_ROWS ? 1.f : in_range(q_scale * k_next * score.mul);
-            float v_scale = v_next;
-            const int64_t row0 = (image0 + t) * ROWS + KEYS * part;
-            const bool by_docs = docs_next;
-            next = walk.from(t + 1);
-            if (next >= 0) {   // a tile ahead: a load takes longer than the waits below should
-                docs_next = !walk.one_document(next);
-                k_next = __ldg(f.k_scale + image0 + next);
-                v_next = __ldg(f.v_scale + image0 + next);
-            }
-            // a warp that gives up still meets the others once, so that none waits for it for good
-            ok = ok && bar_wait_warp(s_full(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_S);
-            fence_after();
-            const uint32_t at = lanes + 128 + 128 * (i & 1) + KEYS * part;
-            float s[KEYS];
-            {
-                uint32_t r[KEYS];
-                tmem_load(at, r);
+            for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+            bool ok = true;
+            auto drain = [&](int i) {   // O of tile i
+                if (!bar_wait_warp(o_full, i & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
+                fence_after();
+                uint32_t r[SHARE];
+                tmem_load(lanes + 384 + part * SHARE, r);
                 tmem_wait_load();
-                if constexpr (BY_ROWS) times_rows(r, f.k_rows + row0, RowFactor(q_scale * score.mul));
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(o_empty);
+                if (v_first != 1.f)
 #pragma unroll
-                for (int c = 0; c < KEYS; c++) s[c] = __uint_as_float(r[c]) * mul;
-            }
-            if constexpr (CAP) {
+                    for (int c = 0; c < SHARE; c++) r[c] = __float_as_uint(__uint_as_float(r[c]) * v_first);
 #pragma unroll
-                for (int c = 0; c < KEYS; c++) s[c] = cap2 * tanh_exact(s[c]);
-            }
-            if constexpr (BIAS) {
-                const float away = float(pos - k0);
-#pragma unroll
-                for (int c = 0; c < KEYS; c++) s[c] = fmaf(-slope2, fabsf(away - float(c)), s[c]);
-            }
-            const int k_last = k0 + KEYS - 1;
-            if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
-                // keys from `ahead` on are hidden by the length or the order
-                const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
-#pragma unroll
-                for (int c = 0; c < KEYS; c++)
-                    if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) s[c] = -INFINITY;
-            }
-            float tops[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int c = 4; c < KEYS; c++) tops[c & 3] = fmaxf(tops[c & 3], s[c]);
-            float* cell = exchange + (i & 1) * PARTS * ROWS;
-            cell[part * ROWS + row] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            if (lane == 0) agreed[SOFTMAX_WARPS * (i & 1) + warp] = ok;
-            row_sync(quad);
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
-            if (!ok) break;
-            // weights in units of the tile's own largest, sums and results in units of the largest so far
-            const float tile_top = row_max(cell, row), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
-            const float from = (tile_top == -INFINITY ? 0.f : tile_top) - P_SHIFT;
-            const float fade = ex2(m - base), unit = ex2(tile_top - base - P_SHIFT);
-            m = top;
-            float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < KEYS; c++) {
-                s[c] = ex2(s[c] - from);
-                sums[c & 3] += s[c];
-            }
-            if constexpr (BY_ROWS) {   // the largest weight times unit of a row sets the unit of its weights
-                times_rows(s, f.v_rows + row0, 0.5f);   // (in range whatever the values are)
-                float* units = exchange + 2 * PARTS * ROWS;
-                units[part * ROWS + row] = largest(s);
-                row_sync(quad);
-                const float own = tile_scale(row_max(units, row));
-                v_scale = own * 2.f;
-#pragma unroll
-                for (int c = 0; c < KEYS; c++) s[c] *= 1.f / own;
-            }
-            store_halves<KEYS>(at, s, 1.f);
-            tmem_wait_store();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(p_ready(i & 1));
-            l = fmaf(l, fade, ((sums[0] + sums[1]) + (sums[2] + sums[3])) * unit);
-            if (i > 0) ok = drain(i - 1);
-            keep = fade;
-            // (two steps where the product would be a subnormal number and lose bits of its own)
-            const bool tiny = v_scale < 0x1p-100f;
-            v_first = tiny ? unit : 1.f;
-            v_before = tiny ? v_scale : v_scale * unit;
-        }
-        if (ok && i > 0) ok = drain(i - 1);
-        float* cell = exchange + (i & 1) * PARTS * ROWS;   // (the last tile's may still be being read)
-        cell[part * ROWS + row] = l;
-        row_sync(quad);
-        if (ok) {
-            l = row_sum(cell, row);
-            if (q < tq) {
-                const bool any = on && l != 0.f;
-                if (gridDim.y > 1) {   // a share of the keys: joined with the others later
-                    float* p = f.partial + ((((int64_t(b) * tq + q) * heads + h) * gridDim.y) + blockIdx.y) * (dim + 2);
-                    if (!any)
-#pragma unroll
-                        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-                    store_row_part<SHARE>(p, part * SHARE, dim, false, acc, 1.f);
-                    if (part == 0) {
-                        p[dim] = any ? m : -INFINITY;
-                        p[dim + 1] = any ? l : 0.f;
-                    }
-                } else if (a.o) {
-                    if (!any)
-#pragma unroll
-                        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-                    store_row_part<SHARE>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
+                for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), v_before, acc[c] * keep);
+                return true;
+            };
+            int i = 0;
+            const int pos_first = q0 + sight.shift;
+            int t = walk.first();
+            bool docs_next = t >= 0 && !walk.one_document(t);
+            float k_next = t >= 0 ? __ldg(f.k_scale + image0 + t) : 0.f, v_next = t >= 0 ? __ldg(f.v_scale + image0 + t) : 0.f;
+            for (int next; t >= 0; t = next, i++) {
+                const int k0 = t * KT + KEYS * part;
+                const float mul = BY_ROWS ? 1.f : in_range(q_scale * k_next * score.mul);
+                float v_scale = v_next;
+                const int64_t row0 = (image0 + t) * ROWS + KEYS * part;
+                const bool by_docs = docs_next;
+                next = walk.from(t + 1);
+                if (next >= 0) {   // a tile ahead: a load takes longer than the waits below should
+                    docs_next = !walk.one_document(next);
+                    k_next = __ldg(f.k_scale + image0 + next);
+                    v_next = __ldg(f.v_scale + image0 + next);
                 }
-                if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + log2f(l) : -INFINITY;
+                // a warp that gives up still meets the others once, so that none waits for it for good
+                ok = ok && bar_wait_warp(s_full(i & 1), (i >> 1) & 1, stop, f.status, GAVE_UP_S);
+                fence_after();
+                const uint32_t at = lanes + 128 + 128 * (i & 1) + KEYS * part;
+                float s[KEYS];
+                {
+                    uint32_t r[KEYS];
+                    tmem_load(at, r);
+                    tmem_wait_load();
+                    if constexpr (BY_ROWS) times_rows(r, f.k_rows + row0, RowFactor(q_scale * score.mul));
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++) s[c] = __uint_as_float(r[c]) * mul;
+                }
+                if constexpr (CAP) {
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++) s[c] = cap2 * tanh_exact(s[c]);
+                }
+                if constexpr (BIAS) {
+                    const float away = float(pos - k0);
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++) s[c] = fmaf(-slope2, fabsf(away - float(c)), s[c]);
+                }
+                const int k_last = k0 + KEYS - 1;
+                if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
+                    // keys from `ahead` on are hidden by the length or the order
+                    const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++)
+                        if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) s[c] = -INFINITY;
+                }
+                float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < KEYS; c++) tops[c & 3] = fmaxf(tops[c & 3], s[c]);
+                float* cell = exchange + (i & 1) * PARTS * ROWS;
+                cell[part * ROWS + row] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                if (lane == 0) agreed[SOFTMAX_WARPS * (i & 1) + warp] = ok;
+                row_sync(quad);
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) ok = ok && agreed[SOFTMAX_WARPS * (i & 1) + 4 * p + quad];
+                if (!ok) break;
+                // weights in units of the tile's own largest, sums and results in units of the largest so far
+                const float tile_top = row_max(cell, row), top = fmaxf(m, tile_top), base = top == -INFINITY ? 0.f : top;
+                const float from = (tile_top == -INFINITY ? 0.f : tile_top) - P_SHIFT;
+                const float fade = ex2(m - base), unit = ex2(tile_top - base - P_SHIFT);
+                m = top;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KEYS; c++) {
+                    s[c] = ex2(s[c] - from);
+                    sums[c & 3] += s[c];
+                }
+                if constexpr (BY_ROWS) {   // the largest weight times unit of a row sets the unit of its weights
+                    times_rows(s, f.v_rows + row0, 0.5f);   // (in range whatever the values are)
+                    float* units = exchange + 2 * PARTS * ROWS;
+                    units[part * ROWS + row] = largest(s);
+                    row_sync(quad);
+                    const float own = tile_scale(row_max(units, row));
+                    v_scale = own * 2.f;
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++) s[c] *= 1.f / own;
+                }
+                store_halves<KEYS>(at, s, 1.f);
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_ready(i & 1));
+                l = fmaf(l, fade, ((sums[0] + sums[1]) + (sums[2] + sums[3])) * unit);
+                if (i > 0) ok = drain(i - 1);
+                keep = fade;
+                // (two steps where the product would be a subnormal number and lose bits of its own)
+                const bool tiny = v_scale < 0x1p-100f;
+                v_first = tiny ? unit : 1.f;
+                v_before = tiny ? v_scale : v_scale * unit;
             }
-        }
+            if (ok && i > 0) ok = drain(i - 1);
+            float* cell = exchange + (i & 1) * PARTS * ROWS;   // (the last tile's may still be being read)
+            cell[part * ROWS + row] = l;
+            row_sync(quad);
+            if (ok) {
+                l = row_sum(cell, row);
+                if (q < tq) {
+                    const bool any = on && l != 0.f;
+                    if (gridDim.y > 1) {   // a share of the keys: joined with the others later
+                        float* p = f.partial + ((((int64_t(b) * tq + q) * heads + h) * gridDim.y) + blockIdx.y) * (dim + 2);
+                        if (!any)
+#pragma unroll
+                            for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+                        store_row_part<SHARE>(p, part * SHARE, dim, false, acc, 1.f);
+                        if (part == 0) {
+                            p[dim] = any ? m : -INFINITY;
+                            p[dim + 1] = any ? l : 0.f;
+                        }
+                    } else if (a.o) {
+                        if (!any)
+#pragma unroll
+                            for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+                        store_row_part<SHARE>(a.o + ((int64_t(b) * tq + q) * heads + h) * dim, part * SHARE, dim, f.o_vec, acc, any ? 1.f / l : 0.f);
+                    }
+                    if (gridDim.y == 1 && a.lse && part == 0) a.lse[int64_t(bh) * tq + q] = any ? m + log2f(l) : -INFINITY;
+                }
+            }
         };
         if (__builtin_expect(by_row[quad] == 0, 1)) arithmetic(std::false_type{});
         else arithmetic(std::true_type{});
@@ -871,100 +871,100 @@ __global__ void __launch_bounds__(THREADS, 1) adb_attention_tc_dq(const GradArgs
         __syncwarp();
         if (lane == 0) bar_arrive(own_ready);
         auto arithmetic = [&](auto units) {
-        constexpr bool BY_ROWS = decltype(units)::value;
-        const ScoreOf score(a, h);
-        float acc[SHARE], factor = 0.f;   // of the accumulator that has not been emptied yet
+            constexpr bool BY_ROWS = decltype(units)::value;
+            const ScoreOf score(a, h);
+            float acc[SHARE], factor = 0.f;   // of the accumulator that has not been emptied yet
 #pragma unroll
-        for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-        bool ok = true;
-        uint32_t n = 0;
-        auto drain = [&](uint32_t tile) {
-            if (!bar_wait_warp(acc_full, tile & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
-            fence_after();
-            uint32_t r[SHARE];
-            tmem_load(lanes + C_DQ + part * SHARE, r);
-            tmem_wait_load();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(acc_taken);
+            for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+            bool ok = true;
+            uint32_t n = 0;
+            auto drain = [&](uint32_t tile) {
+                if (!bar_wait_warp(acc_full, tile & 1, stop, f.status, GAVE_UP_O_FULL)) return false;
+                fence_after();
+                uint32_t r[SHARE];
+                tmem_load(lanes + C_DQ + part * SHARE, r);
+                tmem_wait_load();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(acc_taken);
 #pragma unroll
-            for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), factor, acc[c]);
-            return true;
-        };
-        const int pos_first = q0 + sight.shift;
-        int t = walk.first();
-        bool docs_next = t >= 0 && !walk.one_document(t);
-        float k_next = t >= 0 ? __ldg(f.k.scale + image0 + (t >> 1)) : 0.f, v_next = t >= 0 ? __ldg(f.v.scale + image0 + (t >> 1)) : 0.f;
-        for (int next; t >= 0; t = next, n++) {
-            const int k0 = t * GT + KEYS * part;
-            const bool by_docs = docs_next;
-            const float k_scale = BY_ROWS ? 1.f / ROW_TOP : k_next;
-            const float mul = BY_ROWS ? 1.f : in_range(own_scale[0] * k_next * score.mul), dp_mul = BY_ROWS ? 1.f : in_range(own_scale[1] * v_next);
-            const int64_t row0 = image0 * ROWS + t * GT + KEYS * part;
-            next = walk.from(t + 1);
-            if (next >= 0) {   // a tile ahead
-                docs_next = !walk.one_document(next);
-                k_next = __ldg(f.k.scale + image0 + (next >> 1));
-                v_next = __ldg(f.v.scale + image0 + (next >> 1));
-            }
-            float p[KEYS];   // weights, times the scores' bend
-            uint32_t r[KEYS];
-            if (!bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
-            fence_after();
-            tmem_load(lanes + C_S + KEYS * part, r);
-            tmem_wait_load();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(s_taken);
-            if constexpr (BY_ROWS) times_rows(r, f.k.rows + row0, RowFactor(own_scale[0] * score.mul));
-#pragma unroll
-            for (int c = 0; c < KEYS; c++) {
-                float s = __uint_as_float(r[c]) * mul, bend = 1.f;
-                if constexpr (CAP) {
-                    const float w = tanh_exact(s);
-                    bend = fmaf(-w, w, 1.f);
-                    s = score.cap2 * w;
+                for (int c = 0; c < SHARE; c++) acc[c] = fmaf(__uint_as_float(r[c]), factor, acc[c]);
+                return true;
+            };
+            const int pos_first = q0 + sight.shift;
+            int t = walk.first();
+            bool docs_next = t >= 0 && !walk.one_document(t);
+            float k_next = t >= 0 ? __ldg(f.k.scale + image0 + (t >> 1)) : 0.f, v_next = t >= 0 ? __ldg(f.v.scale + image0 + (t >> 1)) : 0.f;
+            for (int next; t >= 0; t = next, n++) {
+                const int k0 = t * GT + KEYS * part;
+                const bool by_docs = docs_next;
+                const float k_scale = BY_ROWS ? 1.f / ROW_TOP : k_next;
+                const float mul = BY_ROWS ? 1.f : in_range(own_scale[0] * k_next * score.mul), dp_mul = BY_ROWS ? 1.f : in_range(own_scale[1] * v_next);
+                const int64_t row0 = image0 * ROWS + t * GT + KEYS * part;
+                next = walk.from(t + 1);
+                if (next >= 0) {   // a tile ahead
+                    docs_next = !walk.one_document(next);
+                    k_next = __ldg(f.k.scale + image0 + (next >> 1));
+                    v_next = __ldg(f.v.scale + image0 + (next >> 1));
                 }
-                if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(pos - k0 - c)), s);
-                p[c] = CAP ? ex2(s - lse) * bend : ex2(s - lse);
+                float p[KEYS];   // weights, times the scores' bend
+                uint32_t r[KEYS];
+                if (!bar_wait_warp(s_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
+                fence_after();
+                tmem_load(lanes + C_S + KEYS * part, r);
+                tmem_wait_load();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(s_taken);
+                if constexpr (BY_ROWS) times_rows(r, f.k.rows + row0, RowFactor(own_scale[0] * score.mul));
+#pragma unroll
+                for (int c = 0; c < KEYS; c++) {
+                    float s = __uint_as_float(r[c]) * mul, bend = 1.f;
+                    if constexpr (CAP) {
+                        const float w = tanh_exact(s);
+                        bend = fmaf(-w, w, 1.f);
+                        s = score.cap2 * w;
+                    }
+                    if constexpr (BIAS) s = fmaf(-score.slope2, fabsf(float(pos - k0 - c)), s);
+                    p[c] = CAP ? ex2(s - lse) * bend : ex2(s - lse);
+                }
+                const int k_last = k0 + KEYS - 1;
+                if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
+                    const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
+#pragma unroll
+                    for (int c = 0; c < KEYS; c++)
+                        if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) p[c] = 0.f;
+                }
+                if (n > 0) ok = drain(n - 1);     // beside the product dP
+                if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
+                fence_after();
+                tmem_load(lanes + C_DP + KEYS * part, r);
+                tmem_wait_load();
+                if constexpr (BY_ROWS) times_rows(r, f.v.rows + row0, RowFactor(own_scale[1]));
+#pragma unroll
+                for (int c = 0; c < KEYS; c++) {
+                    p[c] = p[c] == 0.f ? 0.f : p[c] * fmaf(__uint_as_float(r[c]), dp_mul, -delta);
+                }
+                if constexpr (BY_ROWS) times_rows(p, f.k.rows + row0, ROW_TOP);
+                float most = 0.f;   // (an infinity may set the unit: it reaches every element of the row's sum anyway)
+#pragma unroll
+                for (int c = 0; c < KEYS; c++) most = fmaxf(most, fabsf(p[c]));
+                if (!row_largest(most, exchange, meet + 8 * quad, n, part, row, stop, f.status)) { ok = false; break; }
+                const float unit = tile_scale(most);
+                factor = unit * k_scale;   // (powers of two: exact down to 2^-149)
+                store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f / unit);
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(ds_ready);
             }
-            const int k_last = k0 + KEYS - 1;
-            if (k_last >= sight.n || by_docs || (sight.causal && k_last > pos_first && k_last >= sight.prefix)) {
-                const int ahead = (sight.causal ? min(sight.n, max(pos + 1, sight.prefix)) : sight.n) - k0;
+            if (ok && n > 0) ok = drain(n - 1);
+            if (ok && q < tq) {
+                if (!on)
 #pragma unroll
-                for (int c = 0; c < KEYS; c++)
-                    if (c >= ahead || (by_docs && __ldg(sight.docs + k0 + c) != doc)) p[c] = 0.f;
+                    for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
+                store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, a.scale);
             }
-            if (n > 0) ok = drain(n - 1);     // beside the product dP
-            if (!ok || !bar_wait_warp(dp_full, n & 1, stop, f.status, GAVE_UP_S)) { ok = false; break; }
-            fence_after();
-            tmem_load(lanes + C_DP + KEYS * part, r);
-            tmem_wait_load();
-            if constexpr (BY_ROWS) times_rows(r, f.v.rows + row0, RowFactor(own_scale[1]));
-#pragma unroll
-            for (int c = 0; c < KEYS; c++) {
-                p[c] = p[c] == 0.f ? 0.f : p[c] * fmaf(__uint_as_float(r[c]), dp_mul, -delta);
-            }
-            if constexpr (BY_ROWS) times_rows(p, f.k.rows + row0, ROW_TOP);
-            float most = 0.f;   // (an infinity may set the unit: it reaches every element of the row's sum anyway)
-#pragma unroll
-            for (int c = 0; c < KEYS; c++) most = fmaxf(most, fabsf(p[c]));
-            if (!row_largest(most, exchange, meet + 8 * quad, n, part, row, stop, f.status)) { ok = false; break; }
-            const float unit = tile_scale(most);
-            factor = unit * k_scale;   // (powers of two: exact down to 2^-149)
-            store_halves<KEYS>(lanes + C_DP + KEYS * part, p, 1.f / unit);
-            tmem_wait_store();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(ds_ready);
-        }
-        if (ok && n > 0) ok = drain(n - 1);
-        if (ok && q < tq) {
-            if (!on)
-#pragma unroll
-                for (int c = 0; c < SHARE; c++) acc[c] = 0.f;
-            store_row_part<SHARE>(f.dq + ((int64_t(blockIdx.y) * a.s.batch + b) * tq + q) * heads * dim + h * dim, part * SHARE, dim, f.out_vec, acc, a.scale);
-        }
         };
         if (__builtin_expect(by_row[quad] == 0, 1)) arithmetic(std::false_type{});
         else arithmetic(std::true_type{});
